@@ -196,8 +196,114 @@ int oumu_attn_prefill_kv(const void *qkv, void *out, void *kc, void *vc, int T, 
                          int maxlen, float scale, oumu_stream_t stream);
 
 /*
+ * ---- The 4-bit paged KV cache -------------------------------------------------------------------------------------
+ *
+ * No counterpart in the reference, whose slots are bf16 and as long as the longest take may become (src/model.rs:
+ * 130-133). Here a take's K and V lie in pages of OUMU_KV4_PAGE positions, handed out as the take grows, shared by
+ * takes that started from one prompt, and hold 5 bits a value (4 and its share of scales): 0.31 of the bf16 bytes, in
+ * memory and in what a decode step reads.
+ *
+ *   pool   [npages][oumu_kv4_page_bytes(nk, hd)] bytes per layer, 16-byte aligned; contents are this library's
+ *   table  int32 [B][maxpages], one for all layers: take s's page of positions [64 k, 64 k + 64) is table[s][k], in
+ *          [0, npages), or -1 for none. A row is filled from the front, without gaps.
+ *   ref    int32 [npages]: how many table entries name a page (0: free)
+ *   lens   int32 [B]: positions of a take; 0 for a take that holds nothing
+ *
+ * A value x of a group (32 consecutive channels of one position of one kv head) is held as n in 0..15 and stands for
+ * s * n + z: z the group's minimum, s the smallest bf16 >= (max - min) / 15, n = (x - z) / s to the nearest, half to
+ * even, so it is within s / 2 of x. A group that holds a NaN or an infinity, or whose spread overflows fp32, reads back
+ * as NaN throughout.
+ *
+ * What is read on the device is checked there: a position no table entry has a page for, an entry outside
+ * [0, npages), a take outside [0, B) sets OUMU_DEVERR_PAGE (4), a length or position outside the table's
+ * [0, 64 maxpages] sets OUMU_DEVERR_LENGTH (2) in the word of oumu_device_error; nothing is read or written out of
+ * range, and the outputs of the takes concerned are unspecified. A page that more than one take holds (ref > 1) must
+ * not be written: oumu_pages_fork shares full pages only, so a take that only grows never does.
+ * B <= 4096 and 64 * maxpages < 2^31 throughout, else OUMU_ERR_UNSUPPORTED.
+ */
+#define OUMU_KV4_PAGE 64
+
+/* Bytes of one page: 160 nk per position at hd 128, 80 nk at hd 64; 0 for other head sizes or nk < 1. */
+size_t oumu_kv4_page_bytes(int nk, int hd);
+
+/*
+ * Quantise k and v (already rotated) into the takes' pages: row s * rows + i of qkv, i < min(count[s], rows)
+ * (count NULL: rows), goes to position start[s] + i (start NULL: i) of take s. The table must have the pages. Rows
+ * from count[s] on are not read, other positions are left as they are. nq may be 0 for a k|v buffer. Takes the place
+ * of oumu_kv_write (kernels/voxcpm.cu:117-129).
+ */
+int oumu_kv4_write(const void *qkv, void *pool, const int *table, const int *start, const int *count, int B, int rows,
+                   int nq, int nk, int hd, int npages, int maxpages, oumu_stream_t stream);
+
+/*
+ * The values the cache stands for, rounded to bf16, into slots kc, vc [B][nk][maxlen][hd]: positions < lens[s] (or
+ * <= *pos) of every take; other positions are left as they are. For the bf16 kernels of this header.
+ */
+int oumu_kv4_read(const void *pool, const int *table, const int *lens, const int *pos, void *kc, void *vc, int B,
+                  int nk, int hd, int npages, int maxpages, int maxlen, oumu_stream_t stream);
+
+/*
+ * oumu_attn_decode over the 4-bit cache: out[s] = softmax(scale * q K^T) V over the first lens[s] (or *pos + 1)
+ * positions, with the K and V the cache stands for, fp32 softmax and sums, one rounding to bf16. A take of length 0
+ * gets zeros. hd in {64, 128}, nq / nk in 1..8. The workspace is zero-filled before its first use (or
+ * oumu_attn_decode_reset with the same B and nk), every call leaves its counters zero, and calls that may overlap
+ * have one each.
+ */
+size_t oumu_attn_decode_kv4_workspace(int B, int nq, int nk, int hd, int maxpages);
+int oumu_attn_decode_kv4(const void *qkv, const void *pool, void *out, void *workspace, size_t workspace_bytes,
+                         const int *table, const int *pos, const int *lens, int B, int nq, int nk, int hd, int npages,
+                         int maxpages, float scale, oumu_stream_t stream);
+
+/*
+ * oumu_attn_decode_step over the 4-bit cache: in one launch, every take's newest position (lens[s] - 1, or *pos) has
+ * its k rotated (cos_t, sin_t [>= that position + 1][hd / 2]; NULL for no rope), k and v quantised into its page, and
+ * its q rotated and attended over positions up to and including it, all as the cache stands for them: the output of
+ * oumu_rope, oumu_kv4_write and oumu_attn_decode_kv4, bit for bit. qkv is not modified. held: bf16 [B][2 nk hd] or
+ * NULL, receives what the cache now holds of the newest k (heads), then v; zeros for a take of length 0.
+ */
+int oumu_attn_decode_kv4_step(const void *qkv, void *pool, void *out, void *held, void *workspace,
+                              size_t workspace_bytes, const float *cos_t, const float *sin_t, const int *table,
+                              const int *pos, const int *lens, int B, int nq, int nk, int hd, int npages,
+                              int maxpages, float scale, oumu_stream_t stream);
+
+/*
+ * Pages of a cache, for any contents: the pool of layer l is `pools` + l * layer_stride, npages pages of page_bytes
+ * (both multiples of 16). They read and change tables on the device, in an order that does not depend on timing, and
+ * can be captured; launches on one table and ref must be ordered with each other.
+ *
+ * extend: every take with lens[s] > 0 gets the pages it lacks for its first lens[s] + extra positions (a step appends
+ * with extra 0 once lens counts the newest position): free pages, lowest first, in the order of takes and positions.
+ * status[0] = pages that were missing because the pool had run out (0: every take has what it needs).
+ *
+ * fork: for i < n, take dst[i] gives its pages back and continues where take src[i] is: it shares the source's full
+ * pages, and its own copy of the last, partly filled one (the lowest free pages, in the order of i) in every layer;
+ * lens[dst[i]] = lens[src[i]]. A pair whose takes are out of range or the same, whose dst an earlier pair has, or
+ * whose src is some pair's dst is not carried out and sets OUMU_DEVERR_PAGE. status[0] = pages missing; the takes they
+ * were missing for end up empty (length 0). Takes the place of oumu_kv_replicate (kernels/voxcpm.cu:407-413) without
+ * writing the prompt once per take. n <= 4096.
+ *
+ * free: takes[i], i < n, give their pages back: row -1, length 0. A take may be listed twice.
+ *
+ * compact: with m pages in use, the k-th of those numbered m or above moves to the k-th free page below m, in every
+ * layer and table row, so that pages m .. npages - 1 are free and the end of the pools can be given back.
+ * status[0] = m, status[1] = pages moved. The workspace (oumu_pages_workspace bytes) needs no initial value.
+ */
+int oumu_pages_extend(int *table, int *ref, const int *lens, int extra, int *status, int B, int npages, int maxpages,
+                      oumu_stream_t stream);
+int oumu_pages_fork(void *pools, long layer_stride, int layers, long page_bytes, int *table, int *ref, int *lens,
+                    const int *src, const int *dst, int n, int *status, int B, int npages, int maxpages,
+                    oumu_stream_t stream);
+int oumu_pages_free(int *table, int *ref, int *lens, const int *takes, int n, int B, int npages, int maxpages,
+                    oumu_stream_t stream);
+size_t oumu_pages_workspace(int npages);
+int oumu_pages_compact(void *pools, long layer_stride, int layers, long page_bytes, int *table, int *ref,
+                       void *workspace, size_t workspace_bytes, int *status, int B, int npages, int maxpages,
+                       oumu_stream_t stream);
+
+/*
  * Device-side error word of this library on the current device: 0 when no kernel recorded an error (a bounded
- * wait that ran out, a length outside [1, maxlen]). Synchronises the device. reset != 0 clears it.
+ * wait that ran out, a length outside [1, maxlen], a page that a table does not have). Synchronises the device.
+ * reset != 0 clears it.
  */
 int oumu_device_error(int reset);
 

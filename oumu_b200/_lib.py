@@ -33,6 +33,17 @@ SIGNATURES = {
     "oumu_attn_full_rope": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "oumu_kv_replicate": (_I, [_P, _I, _I, _I, _I, _I, _P]),
     "oumu_attn_prefill_kv": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
+    "oumu_kv4_page_bytes": (_Z, [_I, _I]),
+    "oumu_kv4_write": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "oumu_kv4_read": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
+    "oumu_attn_decode_kv4_workspace": (_Z, [_I, _I, _I, _I, _I]),
+    "oumu_attn_decode_kv4": (_I, [_P, _P, _P, _P, _Z, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
+    "oumu_attn_decode_kv4_step": (_I, [_P, _P, _P, _P, _P, _Z, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
+    "oumu_pages_extend": (_I, [_P, _P, _P, _I, _P, _I, _I, _I, _P]),
+    "oumu_pages_fork": (_I, [_P, _L, _I, _L, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
+    "oumu_pages_free": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P]),
+    "oumu_pages_workspace": (_Z, [_I]),
+    "oumu_pages_compact": (_I, [_P, _L, _I, _L, _P, _P, _P, _Z, _P, _I, _I, _I, _P]),
     "oumu_device_error": (_I, [_I]),
     "oumu_set_pdl": (_I, [_I]),
     "oumu_set_wait_limit_ns": (_I, [ctypes.c_ulonglong]),

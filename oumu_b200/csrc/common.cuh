@@ -11,6 +11,7 @@ typedef __nv_bfloat16 bf16;
 // Device error word (one per device that loads the library). Codes are OR-ed in, read by oumu_device_error.
 #define OUMU_DEVERR_TIMEOUT 1u   // a bounded wait ran out
 #define OUMU_DEVERR_LENGTH 2u    // a position / length outside [1, maxlen]
+#define OUMU_DEVERR_PAGE 4u      // a page table entry that names no page, a take that is none
 // Defined here: the library is one translation unit (oumu_attn.cu includes every kernel header).
 __device__ unsigned int oumu_dev_error = 0;
 

@@ -14,9 +14,12 @@
 
 #include "common.cuh"
 #include "decode.cuh"
+#include "decode_kv4.cuh"
 #include "feeders.cuh"
 #include "full_small.cuh"
 #include "gemm_tc.cuh"
+#include "kv4.cuh"
+#include "pages.cuh"
 #include "prefill_tc.cuh"
 #include "prefill_pp.cuh"
 #include "small_tc.cuh"
@@ -905,6 +908,216 @@ int oumu_device_error(int reset) {
         OUMU_CK(cudaMemcpyToSymbol(oumu_dev_error, &z, sizeof(z)));
     }
     return static_cast<int>(v);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------------------------
+// The 4-bit paged KV cache
+// ------------------------------------------------------------------------------------------------------------
+
+namespace {
+// Limits every entry point of the paged cache shares.
+int paged_limits(int B, int npages, int maxpages) {
+    if (B < 1 || npages < 1 || maxpages < 1) return OUMU_ERR_INVALID;
+    if (B > pg::BMAX || static_cast<long>(maxpages) * kv4::PAGE >= (1L << 31)) return OUMU_ERR_UNSUPPORTED;
+    return OUMU_OK;
+}
+
+// 8-warp CTAs of one warp per (take, block of 8 positions, kv head, K or V); 0 where the grid would be too large.
+unsigned kv4_grid(int B, long blocks, int nk) {
+    const long ctas = (static_cast<long>(B) * blocks * 2 * nk + 7) / 8;
+    return ctas <= 0x7fffffffL ? static_cast<unsigned>(ctas) : 0u;
+}
+
+size_t kv4_part_bytes(int hd) { return 2 * (2 * static_cast<size_t>(d4::GMAX) + d4::GMAX * hd) * 4; }
+
+template <int HD, bool FUSED>
+int launch_decode_kv4(const d4::Params &P, cudaStream_t st) {
+    const int smem = d4::NW * (2 * d4::GMAX + d4::GMAX * HD) * 4;
+    OUMU_CK(launch_k(d4::k_attn_decode_kv4<HD, FUSED>, dim3(static_cast<unsigned>(P.B * P.nk)), dim3(d4::NW * 32), smem,
+                     st, P));
+    return OUMU_OK;
+}
+
+int decode_kv4_entry(bool fused, const void *qkv, void *pool, void *out, void *held, void *ws, size_t ws_bytes,
+                     const float *cos_t, const float *sin_t, const int *table, const int *pos, const int *lens, int B,
+                     int nq, int nk, int hd, int npages, int maxpages, float scale, oumu_stream_t stream) {
+    if (!qkv || !pool || !out || !ws || !table || (!pos && !lens)) return OUMU_ERR_INVALID;
+    if (nq < 1 || nk < 1 || nq % nk || !(scale > 0.f)) return OUMU_ERR_INVALID;
+    if ((cos_t == nullptr) != (sin_t == nullptr)) return OUMU_ERR_INVALID;
+    int rc = paged_limits(B, npages, maxpages);
+    if (rc) return rc;
+    if (!head_dim_ok(hd) || nq / nk > d4::GMAX) return OUMU_ERR_UNSUPPORTED;
+    if (static_cast<long>(B) * nk * maxpages * 2 >= (1L << 31)) return OUMU_ERR_UNSUPPORTED;
+    if (!aligned16(qkv) || !aligned16(pool) || !aligned16(out) || !aligned16(ws) || (held && !aligned16(held)) ||
+        (cos_t && (!aligned16(cos_t) || !aligned16(sin_t))))
+        return OUMU_ERR_INVALID;
+    const size_t cbytes = decode_counter_bytes(B, nk);
+    if (ws_bytes < cbytes + kv4_part_bytes(hd)) return OUMU_ERR_WORKSPACE;
+    int sms = 0;
+    rc = current_device(&sms);
+    if (rc) return rc;
+    d4::Params P;
+    P.qkv = static_cast<const bf16 *>(qkv);
+    P.pool = static_cast<uint8_t *>(pool);
+    P.table = table;
+    P.out = static_cast<bf16 *>(out);
+    P.held = static_cast<bf16 *>(held);
+    P.cnt = static_cast<int *>(ws);
+    P.part = reinterpret_cast<float *>(static_cast<char *>(ws) + cbytes);
+    P.pos = pos;
+    P.lens = lens;
+    P.cos_t = cos_t;
+    P.sin_t = sin_t;
+    P.B = B;
+    P.nq = nq;
+    P.nk = nk;
+    P.npages = npages;
+    P.maxpages = maxpages;
+    P.sl2 = scale * 1.4426950408889634f;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (fused) return hd == 128 ? launch_decode_kv4<128, true>(P, st) : launch_decode_kv4<64, true>(P, st);
+    return hd == 128 ? launch_decode_kv4<128, false>(P, st) : launch_decode_kv4<64, false>(P, st);
+}
+
+// Pools of `layers` layers; layer_stride only matters from the second on.
+bool pools_ok(const void *pools, long layer_stride, int layers, long page_bytes, int npages) {
+    return pools && aligned16(pools) && layers >= 1 && layers <= 65535 && page_bytes >= 16 && page_bytes % 16 == 0 &&
+           page_bytes <= (1L << 30) && layer_stride % 16 == 0 &&
+           (layers == 1 || layer_stride >= static_cast<long>(npages) * page_bytes);
+}
+}  // namespace
+
+extern "C" {
+
+size_t oumu_kv4_page_bytes(int nk, int hd) {
+    if (nk < 1 || !head_dim_ok(hd)) return 0;
+    return static_cast<size_t>(nk) * (hd == 128 ? kv4::Fmt<128>::UNIT : kv4::Fmt<64>::UNIT);
+}
+
+int oumu_kv4_write(const void *qkv, void *pool, const int *table, const int *start, const int *count, int B, int rows,
+                   int nq, int nk, int hd, int npages, int maxpages, oumu_stream_t stream) {
+    if (!qkv || !pool || !table || rows < 0 || nq < 0 || nk < 1) return OUMU_ERR_INVALID;
+    int rc = paged_limits(B, npages, maxpages);
+    if (rc) return rc;
+    if (!head_dim_ok(hd)) return OUMU_ERR_UNSUPPORTED;
+    if (!aligned16(qkv) || !aligned16(pool)) return OUMU_ERR_INVALID;
+    if (!start && !count && rows > static_cast<long>(maxpages) * kv4::PAGE) return OUMU_ERR_INVALID;
+    if (rows == 0) return OUMU_OK;
+    const int blocks = (rows + 7) / 8 + (start ? 1 : 0);
+    const unsigned grid = kv4_grid(B, blocks, nk);
+    if (!grid) return OUMU_ERR_UNSUPPORTED;
+    auto kern = hd == 128 ? kv4::k_kv4_write<128> : kv4::k_kv4_write<64>;
+    kern<<<grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(static_cast<const bf16 *>(qkv),
+                                                                   static_cast<uint8_t *>(pool), table, start, count, B,
+                                                                   rows, nq, nk, npages, maxpages, blocks);
+    OUMU_CK(cudaGetLastError());
+    return OUMU_OK;
+}
+
+int oumu_kv4_read(const void *pool, const int *table, const int *lens, const int *pos, void *kc, void *vc, int B,
+                  int nk, int hd, int npages, int maxpages, int maxlen, oumu_stream_t stream) {
+    if (!pool || !table || (!lens && !pos) || !kc || !vc || nk < 1 || maxlen < 1) return OUMU_ERR_INVALID;
+    int rc = paged_limits(B, npages, maxpages);
+    if (rc) return rc;
+    if (!head_dim_ok(hd)) return OUMU_ERR_UNSUPPORTED;
+    if (!aligned16(pool) || !aligned16(kc) || !aligned16(vc)) return OUMU_ERR_INVALID;
+    const long span = std::min(static_cast<long>(maxlen), static_cast<long>(maxpages) * kv4::PAGE);
+    const int blocks = static_cast<int>((span + 7) / 8);
+    const unsigned grid = kv4_grid(B, blocks, nk);
+    if (!grid) return OUMU_ERR_UNSUPPORTED;
+    auto kern = hd == 128 ? kv4::k_kv4_read<128> : kv4::k_kv4_read<64>;
+    kern<<<grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+        static_cast<uint8_t *>(const_cast<void *>(pool)), table, lens, pos, static_cast<bf16 *>(kc),
+        static_cast<bf16 *>(vc), B, nk, npages, maxpages, maxlen, blocks);
+    OUMU_CK(cudaGetLastError());
+    return OUMU_OK;
+}
+
+size_t oumu_attn_decode_kv4_workspace(int B, int nq, int nk, int hd, int maxpages) {
+    if (paged_limits(B, 1, maxpages) || nk < 1 || nq < 1 || nq % nk || nq / nk > d4::GMAX || !head_dim_ok(hd)) return 0;
+    int sms = 0;
+    if (current_device(&sms) != OUMU_OK) sms = 160;
+    return decode_counter_bytes(B, nk) + static_cast<size_t>(sms) * kv4_part_bytes(hd);
+}
+
+int oumu_attn_decode_kv4(const void *qkv, const void *pool, void *out, void *workspace, size_t workspace_bytes,
+                         const int *table, const int *pos, const int *lens, int B, int nq, int nk, int hd, int npages,
+                         int maxpages, float scale, oumu_stream_t stream) {
+    return decode_kv4_entry(false, qkv, const_cast<void *>(pool), out, nullptr, workspace, workspace_bytes, nullptr,
+                            nullptr, table, pos, lens, B, nq, nk, hd, npages, maxpages, scale, stream);
+}
+
+int oumu_attn_decode_kv4_step(const void *qkv, void *pool, void *out, void *held, void *workspace,
+                              size_t workspace_bytes, const float *cos_t, const float *sin_t, const int *table,
+                              const int *pos, const int *lens, int B, int nq, int nk, int hd, int npages,
+                              int maxpages, float scale, oumu_stream_t stream) {
+    return decode_kv4_entry(true, qkv, pool, out, held, workspace, workspace_bytes, cos_t, sin_t, table, pos, lens, B,
+                            nq, nk, hd, npages, maxpages, scale, stream);
+}
+
+int oumu_pages_extend(int *table, int *ref, const int *lens, int extra, int *status, int B, int npages, int maxpages,
+                      oumu_stream_t stream) {
+    if (!table || !ref || !lens || !status || extra < 0) return OUMU_ERR_INVALID;
+    int rc = paged_limits(B, npages, maxpages);
+    if (rc) return rc;
+    pg::k_pages_extend<<<1, pg::NT, 0, reinterpret_cast<cudaStream_t>(stream)>>>(table, ref, lens, extra, status, B,
+                                                                                npages, maxpages);
+    OUMU_CK(cudaGetLastError());
+    return OUMU_OK;
+}
+
+int oumu_pages_fork(void *pools, long layer_stride, int layers, long page_bytes, int *table, int *ref, int *lens,
+                    const int *src, const int *dst, int n, int *status, int B, int npages, int maxpages,
+                    oumu_stream_t stream) {
+    if (!table || !ref || !lens || !status || n < 0 || (n > 0 && (!src || !dst))) return OUMU_ERR_INVALID;
+    int rc = paged_limits(B, npages, maxpages);
+    if (rc) return rc;
+    if (!pools_ok(pools, layer_stride, layers, page_bytes, npages)) return OUMU_ERR_INVALID;
+    if (n > pg::BMAX) return OUMU_ERR_UNSUPPORTED;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    pg::k_pages_fork<<<1, pg::NT, 0, st>>>(table, ref, lens, src, dst, n, status, B, npages, maxpages);
+    OUMU_CK(cudaGetLastError());
+    if (n == 0) return OUMU_OK;
+    pg::k_pages_fork_copy<<<dim3(static_cast<unsigned>(n), static_cast<unsigned>(layers)), 256, 0, st>>>(
+        static_cast<uint8_t *>(pools), layer_stride, page_bytes, table, lens, src, dst, n, B, npages, maxpages);
+    OUMU_CK(cudaGetLastError());
+    return OUMU_OK;
+}
+
+int oumu_pages_free(int *table, int *ref, int *lens, const int *takes, int n, int B, int npages, int maxpages,
+                    oumu_stream_t stream) {
+    if (!table || !ref || !lens || n < 0 || (n > 0 && !takes)) return OUMU_ERR_INVALID;
+    int rc = paged_limits(B, npages, maxpages);
+    if (rc) return rc;
+    if (n == 0) return OUMU_OK;
+    pg::k_pages_free<<<static_cast<unsigned>((static_cast<long>(n) + 7) / 8), 256, 0,
+                       reinterpret_cast<cudaStream_t>(stream)>>>(table, ref, lens, takes, n, B, npages, maxpages);
+    OUMU_CK(cudaGetLastError());
+    return OUMU_OK;
+}
+
+size_t oumu_pages_workspace(int npages) { return npages < 1 ? 0 : pg::Plan::bytes(npages); }
+
+int oumu_pages_compact(void *pools, long layer_stride, int layers, long page_bytes, int *table, int *ref,
+                       void *workspace, size_t workspace_bytes, int *status, int B, int npages, int maxpages,
+                       oumu_stream_t stream) {
+    if (!table || !ref || !workspace || !status || !aligned16(workspace)) return OUMU_ERR_INVALID;
+    int rc = paged_limits(B, npages, maxpages);
+    if (rc) return rc;
+    if (!pools_ok(pools, layer_stride, layers, page_bytes, npages)) return OUMU_ERR_INVALID;
+    if (workspace_bytes < pg::Plan::bytes(npages)) return OUMU_ERR_WORKSPACE;
+    int sms = 0;
+    rc = current_device(&sms);
+    if (rc) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    pg::k_pages_plan<<<1, pg::NT, 0, st>>>(ref, workspace, status, npages);
+    OUMU_CK(cudaGetLastError());
+    pg::k_pages_move<<<static_cast<unsigned>(sms * 8), 256, 0, st>>>(static_cast<uint8_t *>(pools), layer_stride, layers,
+                                                                     page_bytes, table, workspace, B, npages, maxpages);
+    OUMU_CK(cudaGetLastError());
+    return OUMU_OK;
 }
 
 // ------------------------------------------------------------------------------------------------------------

@@ -268,3 +268,156 @@ def attn_prefill_kv(qkv, out, kc, vc, T, slots, nq, nk, hd, maxlen, scale):
     kv_write + attn_full (src/model.rs:553-567) and kv_replicate (src/model.rs:705-717)."""
     _lib.call("oumu_attn_prefill_kv", _p(qkv), _p(out), _p(kc), _p(vc), T, slots, nq, nk, hd, maxlen, float(scale),
               _stream())
+
+
+# ------------------------------------------------------------------------------------------------------------
+# The 4-bit paged KV cache (include/oumu_attn.h). pool: uint8 [npages][page bytes] of one layer; pools: uint8
+# [layers][npages][page bytes]; table: int32 [B][maxpages]; ref: int32 [npages]; lens: int32 [B]; status: int32 [2]
+# ------------------------------------------------------------------------------------------------------------
+
+KV4_PAGE = 64
+
+
+def kv4_page_bytes(nk, hd):
+    n = int(_lib.load().oumu_kv4_page_bytes(nk, hd))
+    if n == 0:
+        raise ValueError("unsupported cache shape")
+    return n
+
+
+def _kv4_check(pool, table, *ints, nk=0, hd=0, B=0):
+    """What the C entry points cannot see of tensors: types, layouts, sizes, the device."""
+    if pool.dtype is not torch.uint8 or not pool.is_contiguous():
+        raise ValueError("pool: a contiguous uint8 tensor")
+    if hd and (pool.dim() != 2 or hd not in HD_SUPPORTED or pool.shape[1] != nk * (2 * KV4_PAGE) * (hd * 5 // 8)):
+        raise ValueError("pool: [npages][kv4_page_bytes(nk, hd)]")
+    if table.dim() != 2 or table.shape[0] < B:
+        raise ValueError("table: [B][maxpages]")
+    dev = torch.cuda.current_device()
+    if pool.get_device() != dev:
+        raise ValueError("the cache is not on the current device")
+    for t in (table, *ints):
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev):
+            raise ValueError("page tables, counts, lengths and takes: contiguous int32 tensors on the current device")
+
+
+def _takes(n, *ts):
+    for t in ts:
+        if t is not None and t.numel() < n:
+            raise ValueError("starts, counts and lengths: one per take")
+
+
+def _rows(t, n, what):
+    if t is not None and (t.dtype.itemsize != 2 or not t.is_contiguous() or t.numel() < n):
+        raise ValueError(f"{what}: contiguous 16-bit rows")
+
+
+def kv4_write(qkv, pool, table, start, count, B, rows, nq, nk, hd):
+    """k and v of qkv rows s * rows + i, i < min(count[s], rows), quantised into take s's pages at start[s] + i
+    (oumu_kv4_write; count None: every row, start None: from 0)."""
+    _kv4_check(pool, table, start, count, nk=nk, hd=hd, B=B)
+    _takes(B, start, count)
+    _rows(qkv, B * rows * (nq + 2 * nk) * hd, "qkv")
+    _lib.call("oumu_kv4_write", _p(qkv), _p(pool), _p(table), _p(start), _p(count), B, rows, nq, nk, hd,
+              pool.shape[0], table.shape[1], _stream())
+
+
+def kv4_read(pool, table, lens, kc, vc, nk, hd, pos=None):
+    """What the cache stands for of positions < lens[s] (or <= *pos), as bf16 slots kc, vc [B][nk][maxlen][hd]
+    (oumu_kv4_read)."""
+    B, maxlen = kc.shape[0], kc.shape[2]
+    _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
+    _takes(B, lens)
+    _rows(kc, B * nk * maxlen * hd, "kc")
+    _rows(vc, B * nk * maxlen * hd, "vc")
+    _lib.call("oumu_kv4_read", _p(pool), _p(table), _p(lens), _p(pos), _p(kc), _p(vc), B, nk, hd, pool.shape[0],
+              table.shape[1], maxlen, _stream())
+
+
+def decode_kv4_workspace(B, nq, nk, hd, maxpages, device=None):
+    """A zero-filled workspace for attn_decode_kv4 and attn_decode_kv4_step."""
+    n = int(_lib.load().oumu_attn_decode_kv4_workspace(B, nq, nk, hd, maxpages))
+    if n == 0:
+        raise ValueError("unsupported decode shape")
+    return torch.zeros(n, dtype=torch.uint8, device=device or "cuda")
+
+
+def attn_decode_kv4(qkv, pool, out, workspace, table, pos, lens, B, nq, nk, hd, scale):
+    """attn_decode over the 4-bit paged cache (oumu_attn_decode_kv4). Lengths: lens[s] or *pos + 1."""
+    _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
+    _takes(B, lens)
+    _rows(qkv, B * (nq + 2 * nk) * hd, "qkv")
+    _rows(out, B * nq * hd, "out")
+    _lib.call("oumu_attn_decode_kv4", _p(qkv), _p(pool), _p(out), _p(workspace), workspace.numel(), _p(table), _p(pos),
+              _p(lens), B, nq, nk, hd, pool.shape[0], table.shape[1], float(scale), _stream())
+
+
+def attn_decode_kv4_step(qkv, pool, out, workspace, cos_t, sin_t, table, pos, lens, B, nq, nk, hd, scale, held=None):
+    """One decode layer over the 4-bit paged cache in one launch: rope, quantisation and cache write of the newest
+    position, then the attention (oumu_attn_decode_kv4_step). held: bf16 [B][2 nk hd], receives what the cache holds
+    of the newest k and v."""
+    _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
+    _takes(B, lens)
+    _rows(qkv, B * (nq + 2 * nk) * hd, "qkv")
+    _rows(out, B * nq * hd, "out")
+    _rows(held, B * 2 * nk * hd, "held")
+    _lib.call("oumu_attn_decode_kv4_step", _p(qkv), _p(pool), _p(out), _p(held), _p(workspace), workspace.numel(),
+              _p(cos_t), _p(sin_t), _p(table), _p(pos), _p(lens), B, nq, nk, hd, pool.shape[0], table.shape[1],
+              float(scale), _stream())
+
+
+def _pools(pools, ref):
+    if pools.dim() != 3 or ref.numel() != pools.shape[1]:
+        raise ValueError("pools: [layers][npages][page bytes], ref: [npages]")
+    return _p(pools), pools.stride(0), pools.shape[0], pools.shape[2]
+
+
+def pages_extend(table, ref, lens, extra, status):
+    """Every take that holds positions gets the pages it lacks for lens[s] + extra of them (oumu_pages_extend);
+    status[0]: pages missing."""
+    dev = torch.cuda.current_device()
+    for t in (table, ref, lens, status):
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev:
+            raise ValueError("page tables, counts, lengths and takes: contiguous int32 tensors on the current device")
+    if table.dim() != 2 or lens.numel() < table.shape[0] or status.numel() < 1:
+        raise ValueError("table: [B][maxpages], lens: [B], status: [1]")
+    _lib.call("oumu_pages_extend", _p(table), _p(ref), _p(lens), extra, _p(status), table.shape[0], ref.numel(),
+              table.shape[1], _stream())
+
+
+def pages_fork(pools, table, ref, lens, src, dst, status):
+    """Take dst[i] continues where take src[i] is: shared full pages, a copy of the last one (oumu_pages_fork);
+    status[0]: pages missing."""
+    _kv4_check(pools, table, ref, lens, src, dst, status)
+    if lens.numel() < table.shape[0] or src.numel() != dst.numel() or status.numel() < 1:
+        raise ValueError("lens: [B], src and dst: one take each per pair, status: [1]")
+    _lib.call("oumu_pages_fork", *_pools(pools, ref), _p(table), _p(ref), _p(lens), _p(src), _p(dst), src.numel(),
+              _p(status), table.shape[0], ref.numel(), table.shape[1], _stream())
+
+
+def pages_free(table, ref, lens, takes):
+    """The takes give their pages back and are empty (oumu_pages_free)."""
+    dev = torch.cuda.current_device()
+    for t in (table, ref, lens, takes):
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev:
+            raise ValueError("page tables, counts, lengths and takes: contiguous int32 tensors on the current device")
+    if table.dim() != 2 or lens.numel() < table.shape[0]:
+        raise ValueError("table: [B][maxpages], lens: [B]")
+    _lib.call("oumu_pages_free", _p(table), _p(ref), _p(lens), _p(takes), takes.numel(), table.shape[0], ref.numel(),
+              table.shape[1], _stream())
+
+
+def pages_workspace(npages, device=None):
+    n = int(_lib.load().oumu_pages_workspace(npages))
+    if n == 0:
+        raise ValueError("a pool has at least one page")
+    return torch.empty(n, dtype=torch.uint8, device=device or "cuda")
+
+
+def pages_compact(pools, table, ref, workspace, status):
+    """Pages in use move to the front of the pools (oumu_pages_compact); status: [pages in use, pages moved]."""
+    _kv4_check(pools, table, ref, status)
+    if status.numel() < 2:
+        raise ValueError("status: [2]")
+    _lib.call("oumu_pages_compact", *_pools(pools, ref), _p(table), _p(ref), _p(workspace), workspace.numel(),
+              _p(status), table.shape[0], ref.numel(), table.shape[1], _stream())
