@@ -142,8 +142,8 @@ struct Query {
             }
         }
         if constexpr (W == 4) {
-            z0 = t < 2 ? part[0][t & 1] : part[1][t & 1];
-            z1 = t < 2 ? part[2][t & 1] : 0u;
+            z0 = t & 1 ? (t < 2 ? part[0][W / 2 - 1] : part[1][W / 2 - 1]) : (t < 2 ? part[0][0] : part[1][0]);
+            z1 = t < 2 ? (t & 1 ? part[2][W / 2 - 1] : part[2][0]) : 0u;
         } else {
             z0 = t == 0 ? part[0][0] : t == 1 ? part[1][0] : t == 2 ? part[2][0] : 0u;
             z1 = 0u;
@@ -304,9 +304,8 @@ struct State {
         }
     }
 
-    // The state as a record: m[8], l[8], o[8][HD] (o with the zeros' term, in the values' own unit).
-    __device__ __forceinline__ void record(float *R, int lane) {
-        const int g = lane >> 2, t = lane & 3;
+    // The lanes' shares of the sum and of the zeros' term, added up over the positions.
+    __device__ __forceinline__ void reduce() {
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
@@ -315,6 +314,35 @@ struct State {
 #pragma unroll
                 for (int w = 0; w < W; w++) z[w][c] += __shfl_xor_sync(0xffffffffu, z[w][c], o);
             }
+    }
+    // Numerators of head 2t + c, channels 32w + 4g .. + 3, with the zeros' term, in the values' own unit.
+    __device__ __forceinline__ float4 numerators(int w, int c) const {
+        const float u = 16777216.f, u16 = 1048576.f;  // 2^24, and / 16 for the odd nibbles
+        return make_float4(fmaf(acc[2 * w][c], u, z[w][c]), fmaf(acc[2 * w][c + 2], u16, z[w][c]),
+                           fmaf(acc[2 * w + 1][c], u, z[w][c]), fmaf(acc[2 * w + 1][c + 2], u16, z[w][c]));
+    }
+    // The output of a segment that this warp has seen whole; out: its first head's row.
+    __device__ __forceinline__ void finish(bf16 *out, int G, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        reduce();
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            if (2 * t + c >= G) continue;
+            const float r = 1.f / l[c];
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const float4 o = numerators(w, c);
+                uint2 u;
+                u.x = pack_bf16x2(o.x * r, o.y * r);
+                u.y = pack_bf16x2(o.z * r, o.w * r);
+                *reinterpret_cast<uint2 *>(out + (2 * t + c) * HD + 32 * w + 4 * g) = u;
+            }
+        }
+    }
+    // The state as a record: m[8], l[8], o[8][HD].
+    __device__ __forceinline__ void record(float *R, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        reduce();
         if (g == 0) {
             R[2 * t] = M[0];
             R[2 * t + 1] = M[1];
@@ -324,77 +352,121 @@ struct State {
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int w = 0; w < W; w++) {
-                const float u = 16777216.f, u16 = 1048576.f;  // 2^24, and / 16 for the odd nibbles
-                *reinterpret_cast<float4 *>(R + 2 * GMAX + (2 * t + c) * HD + 32 * w + 4 * g) =
-                    make_float4(fmaf(acc[2 * w][c], u, z[w][c]), fmaf(acc[2 * w][c + 2], u16, z[w][c]),
-                                fmaf(acc[2 * w + 1][c], u, z[w][c]), fmaf(acc[2 * w + 1][c + 2], u16, z[w][c]));
-            }
+            for (int w = 0; w < W; w++)
+                *reinterpret_cast<float4 *>(R + 2 * GMAX + (2 * t + c) * HD + 32 * w + 4 * g) = numerators(w, c);
     }
 };
 
-// Fused form: the newest position's k (rotated) and v, quantised by one warp into position p of the take's cache, in
-// global memory and in `tile`, the copy of that half in shared memory (null: none). Lane l has channels 4l .. 4l + 3.
+// Fused form: the newest position's k (rotated) and v, quantised by the warp that has the segment's last tile. Lane l has
+// channels 4l .. 4l + 3. `make` writes them into the take's page (and `held`) as soon as q arrives; `patch` into the
+// copy of that half in shared memory, which was on its way already.
 template <int HD>
-__device__ __forceinline__ void newest(const Params &P, int s, int kh, int p, int lane, uint8_t *half, uint8_t *tile) {
-    using F = Fmt<HD>;
-    constexpr int W = F::W;
-    const bool on = lane < HD / 4;
-    const int w = lane >> 3, j = lane & 7, r = p % HALF, c4 = 4 * (on ? lane : 0);
-    const bf16 *row = P.qkv + static_cast<long>(s) * (P.nq + 2 * P.nk) * HD;
+struct Newest {
+    static constexpr int W = Fmt<HD>::W;
+    uint32_t code[2], meta[2];  // K word | V half word; scale | zero << 16
+    __device__ __forceinline__ static int code_at(int kv, int r, int lane) {
+        using F = Fmt<HD>;
+        const int w = lane >> 3, j = lane & 7;
+        return kv == 0 ? r / 8 * F::BLOCK + ((r % 8 * 4 + j / 2) * W + w) * 4
+                       : F::CODES + r / 8 * F::BLOCK + ((j * 4 + r % 8 / 2) * W + w) * 4 + 2 * (r & 1);
+    }
+    __device__ __forceinline__ void patch(uint8_t *half, int r, int lane) const {
+        using F = Fmt<HD>;
+        if (lane >= HD / 4) return;
+        if (!(lane & 1)) *reinterpret_cast<uint32_t *>(half + code_at(0, r, lane)) = code[0];
+        *reinterpret_cast<uint16_t *>(half + code_at(1, r, lane)) = static_cast<uint16_t>(code[1]);
+        if ((lane & 7) == 0) {
 #pragma unroll
-    for (int kv = 0; kv < 2; kv++) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(row + (P.nq + kv * P.nk + kh) * HD + c4);
-        float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
-        float x[4] = {a.x, a.y, b.x, b.y};
-        if (kv == 0 && P.cos_t) {
-            const int i = c4 % (HD / 2);
-            const float4 c = *reinterpret_cast<const float4 *>(P.cos_t + static_cast<long>(p) * (HD / 2) + i);
-            const float4 sn = *reinterpret_cast<const float4 *>(P.sin_t + static_cast<long>(p) * (HD / 2) + i);
-            const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {sn.x, sn.y, sn.z, sn.w};
-            float y[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = __shfl_xor_sync(0xffffffffu, x[e], HD / 8);
-#pragma unroll
-            for (int e = 0; e < 4; e++)  // low half: a c - b s; high half: b c + a s
-                x[e] = bf2f(f2bf(c4 < HD / 2 ? x[e] * cc[e] - y[e] * ss[e] : x[e] * cc[e] + y[e] * ss[e]));
-        }
-        const uint32_t u0 = pack_bf16x2(x[0], x[1]), u1 = pack_bf16x2(x[2], x[3]);
-        uint32_t rg = kv4::range_of(kv4::as_u32(__hmax2_nan(kv4::as_bf2(u0), kv4::as_bf2(u1))),
-                                    kv4::as_u32(__hmin2_nan(kv4::as_bf2(u0), kv4::as_bf2(u1))));
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) rg = kv4::range_max(rg, __shfl_xor_sync(0xffffffffu, rg, o));
-        const kv4::Quant q = kv4::quant_of(rg);
-        uint32_t n[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) n[e] = kv4::quant_code(x[e], q);
-        if (P.held && on) {
-            uint2 o;
-            o.x = pack_bf16x2(fmaf(q.s, n[0], q.z), fmaf(q.s, n[1], q.z));
-            o.y = pack_bf16x2(fmaf(q.s, n[2], q.z), fmaf(q.s, n[3], q.z));
-            *reinterpret_cast<uint2 *>(P.held + (static_cast<long>(s) * 2 * P.nk + kv * P.nk + kh) * HD + c4) = o;
-        }
-        // K: this lane's codes are two bytes of the word of lanes (j, j ^ 1); V: one half of a word
-        uint32_t kw = (n[0] | n[2] << 4 | (n[1] | n[3] << 4) << 16) << (8 * (j & 1));
-        kw |= __shfl_xor_sync(0xffffffffu, kw, 1);
-        const int at = kv == 0 ? r / 8 * F::BLOCK + ((r % 8 * 4 + j / 2) * W + w) * 4
-                               : F::CODES + r / 8 * F::BLOCK + ((j * 4 + r % 8 / 2) * W + w) * 4 + 2 * (r & 1);
-        const int meta = (kv ? F::VMETA : F::KMETA) + r * F::ROW + 2 * w;
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            uint8_t *base = k ? tile : half;
-            if (!base || !on) continue;
-            if (kv) *reinterpret_cast<uint16_t *>(base + at) = static_cast<uint16_t>(n[0] | n[1] << 4 | n[2] << 8 | n[3] << 12);
-            else if (!(j & 1)) *reinterpret_cast<uint32_t *>(base + at) = kw;
-            if (j == 0) {
-                *reinterpret_cast<uint16_t *>(base + meta) = static_cast<uint16_t>(__float_as_uint(q.s) >> 16);
-                *reinterpret_cast<uint16_t *>(base + meta + 2 * W) = static_cast<uint16_t>(__float_as_uint(q.z) >> 16);
+            for (int kv = 0; kv < 2; kv++) {
+                uint8_t *m = half + (kv ? F::VMETA : F::KMETA) + r * F::ROW + 2 * (lane >> 3);
+                *reinterpret_cast<uint16_t *>(m) = static_cast<uint16_t>(meta[kv]);
+                *reinterpret_cast<uint16_t *>(m + 2 * W) = static_cast<uint16_t>(meta[kv] >> 16);
             }
         }
     }
+    __device__ __forceinline__ void make(const Params &P, int s, int kh, int p, int lane, uint8_t *half) {
+        const bool on = lane < HD / 4;
+        const int j = lane & 7, c4 = 4 * (on ? lane : 0);
+        const bf16 *row = P.qkv + static_cast<long>(s) * (P.nq + 2 * P.nk) * HD;
+        uint2 u[2];
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) u[kv] = *reinterpret_cast<const uint2 *>(row + (P.nq + kv * P.nk + kh) * HD + c4);
+        if (P.cos_t) {
+            const float2 a = unpack_bf16x2(u[0].x), b = unpack_bf16x2(u[0].y);
+            const int i = c4 % (HD / 2);
+            const float4 c = *reinterpret_cast<const float4 *>(P.cos_t + static_cast<long>(p) * (HD / 2) + i);
+            const float4 sn = *reinterpret_cast<const float4 *>(P.sin_t + static_cast<long>(p) * (HD / 2) + i);
+            const float x[4] = {a.x, a.y, b.x, b.y}, cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {sn.x, sn.y, sn.z, sn.w};
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {  // low half: a c - b s; high half: b c + a s
+                const float o = __shfl_xor_sync(0xffffffffu, x[e], HD / 8);
+                y[e] = c4 < HD / 2 ? x[e] * cc[e] - o * ss[e] : x[e] * cc[e] + o * ss[e];
+            }
+            u[0].x = pack_bf16x2(y[0], y[1]);
+            u[0].y = pack_bf16x2(y[2], y[3]);
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+            uint32_t rg = kv4::range_of(kv4::as_u32(__hmax2_nan(kv4::as_bf2(u[kv].x), kv4::as_bf2(u[kv].y))),
+                                        kv4::as_u32(__hmin2_nan(kv4::as_bf2(u[kv].x), kv4::as_bf2(u[kv].y))));
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) rg = kv4::range_max(rg, __shfl_xor_sync(0xffffffffu, rg, o));
+            const kv4::Quant q = kv4::quant_of(rg);
+            const float2 a = unpack_bf16x2(u[kv].x), b = unpack_bf16x2(u[kv].y);
+            const uint32_t n[4] = {static_cast<uint32_t>(kv4::quant_code(a.x, q)),
+                                   static_cast<uint32_t>(kv4::quant_code(a.y, q)),
+                                   static_cast<uint32_t>(kv4::quant_code(b.x, q)),
+                                   static_cast<uint32_t>(kv4::quant_code(b.y, q))};
+            if (P.held && on) {
+                uint2 o;
+                o.x = pack_bf16x2(fmaf(q.s, n[0], q.z), fmaf(q.s, n[1], q.z));
+                o.y = pack_bf16x2(fmaf(q.s, n[2], q.z), fmaf(q.s, n[3], q.z));
+                *reinterpret_cast<uint2 *>(P.held + (static_cast<long>(s) * 2 * P.nk + kv * P.nk + kh) * HD + c4) = o;
+            }
+            if (kv == 0) {  // two bytes of the word that lanes j and j ^ 1 share
+                const uint32_t kw = (n[0] | n[2] << 4 | (n[1] | n[3] << 4) << 16) << (8 * (j & 1));
+                code[0] = kw | __shfl_xor_sync(0xffffffffu, kw, 1);
+            } else {
+                code[1] = n[0] | n[1] << 4 | n[2] << 8 | n[3] << 12;
+            }
+            meta[kv] = kv4::meta_bits(q.s, q.z);
+        }
+        patch(half, p % HALF, lane);
+    }
+};
+
+// Work is counted in tiles (halves of 32 positions of one take and kv head, a "segment"), laid end to end take by take
+// and cut into equal contiguous ranges: one per CTA, and that into one per warp. A warp streams its range through a
+// ring of its own in shared memory (one bulk copy of 5 KB per tile, nothing shared, no producer warp), so a CTA keeps
+// NW * ST copies in flight and no warp waits for another before the range's end. A segment that lies inside a warp's
+// range is finished by it alone; the parts of one that crosses warps meet in shared memory, of one that crosses CTAs in
+// records in global memory, where the last to arrive adds them up in CTA order: the result does not depend on timing.
+constexpr int NW = 8;           // warps
+constexpr int ST = 4;           // tiles in flight per warp: 8 x 4 x 5 KB = 160 KB per SM
+constexpr int NT = NW * 32;
+constexpr int MIN_TILES = 2 * NW;  // tiles per CTA at least
+
+template <int HD>
+struct Lay {
+    static constexpr int REC = 2 * GMAX + GMAX * HD;  // floats of a record: m[8], l[8], o[8][HD]
+    static_assert(REC * 4 <= ST * Fmt<HD>::HALFB, "a warp's last record lies in its own ring");
+    static constexpr int RING = ST * Fmt<HD>::HALFB;
+    static constexpr int FIRST = NW * RING;           // records of segments that end inside a warp's range
+    static constexpr int BAR = FIRST + NW * REC * 4;
+    static constexpr int SEG = BAR + NW * ST * 8;     // first segment of each warp: id, start
+    static constexpr int MISC = SEG + NW * 8;
+    static constexpr int PRE = MISC + 64;             // pre[B + 1], lens[B]
+    static __host__ __device__ int bytes(int B) { return PRE + (2 * B + 1) * 4; }
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
-// Length of take s: lens[s] or *pos + 1, cut to what its table row can hold (recorded).
+// Take s's length: lens[s] or *pos + 1, cut to what its table row can hold (recorded).
 __device__ __forceinline__ int take_len(const Params &P, int s) {
     int L = P.lens ? P.lens[s] : *P.pos + 1;
     const int room = P.maxpages * kv4::PAGE;
@@ -404,59 +476,252 @@ __device__ __forceinline__ int take_len(const Params &P, int s) {
     }
     return L;
 }
+__device__ __forceinline__ int tiles_of(int L) { return (L + HALF - 1) / HALF; }
 
-constexpr int NW = 8;  // warps of a CTA
+// The take whose tiles hold tile t: the last s with pre[s] <= t (takes without tiles are passed over).
+__device__ __forceinline__ int take_of(const int *pre, int B, int t) {
+    int lo = 0, hi = B - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pre[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+__device__ __forceinline__ int cut(int i, int n, int W) {  // start of part i of W tiles in n parts
+    return static_cast<int>(static_cast<long>(i) * W / n);
+}
 
-// One CTA per (take, kv head): its warps take the tiles in turn, each with a state of its own, merged at the end.
 template <int HD, bool FUSED>
-__global__ void __launch_bounds__(NW * 32) k_attn_decode_kv4(Params P) {
+__global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
     using F = Fmt<HD>;
-    constexpr int REC = 2 * GMAX + GMAX * HD;
-    extern __shared__ __align__(16) float recs[];
-    const int s = blockIdx.x / P.nk, kh = blockIdx.x % P.nk, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = P.nq / P.nk;
+    using Y = Lay<HD>;
+    extern __shared__ __align__(128) uint8_t sm[];
+    int *pre = reinterpret_cast<int *>(sm + Y::PRE), *Ls = pre + P.B + 1;
+    int *misc = reinterpret_cast<int *>(sm + Y::MISC);
+    int2 *segs = reinterpret_cast<int2 *>(sm + Y::SEG);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int B = P.B, nk = P.nk, G = P.nq / P.nk, c = blockIdx.x;
+    const uint32_t ring = smem_u32(sm) + warp * Y::RING, bars = smem_u32(sm) + Y::BAR + warp * ST * 8;
+
+    if (lane < ST) mbar_init(bars + 8 * lane, 1);
+    mbar_fence_init();
     pdl_trigger();
     pdl_wait();
-    const int L = take_len(P, s);
-    bf16 *out = P.out + (static_cast<long>(s) * P.nq + kh * G) * HD;
-    if (L == 0) {
-        for (int i = threadIdx.x; i < G * HD; i += NW * 32) out[i] = f2bf(0.f);
-        if (FUSED && P.held)
-            for (int i = threadIdx.x; i < 2 * HD; i += NW * 32)
-                P.held[(static_cast<long>(s) * 2 * P.nk + i / HD * P.nk + kh) * HD + i % HD] = f2bf(0.f);
-        return;
-    }
-    Query<HD> Q;
-    Q.load(P, s, kh, L - 1, lane);
-    State<HD> S;
-    S.clear();
-    const int tiles = (L + HALF - 1) / HALF;
-    for (int j = warp; j < tiles; j += NW) {
-        int page = P.table[static_cast<long>(s) * P.maxpages + j / 2];
-        if (page < 0 || page >= P.npages) {
-            if (lane == 0) record_error(OUMU_DEVERR_PAGE);
-            continue;
+    // tiles before every take
+    {
+        int run = 0;
+        for (int s0 = 0; s0 < B; s0 += NT) {
+            const int s = s0 + threadIdx.x, L = s < B ? take_len(P, s) : 0, n = tiles_of(L) * nk;
+            int x = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            if (lane == 31) misc[warp] = x;
+            __syncthreads();
+            int before = run, all = run;
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                before += w < warp ? misc[w] : 0;
+                all += misc[w];
+            }
+            if (s < B) {
+                pre[s] = before + x - n;
+                Ls[s] = L;
+            }
+            run = all;
+            __syncthreads();
         }
-        uint8_t *half = P.pool + (static_cast<long>(page) * P.nk + kh) * F::UNIT + (j & 1) * F::HALFB;
-        if (FUSED && j == tiles - 1) {
-            newest<HD>(P, s, kh, L - 1, lane, half, nullptr);
-            __syncwarp();
-        }
-        S.tile(half, L - j * HALF, Q, lane);
+        if (threadIdx.x == 0) pre[B] = run;
     }
-    S.record(recs + warp * REC, lane);
     __syncthreads();
-    for (int i = threadIdx.x; i < G * HD; i += NW * 32) {
-        const int h = i / HD;
-        float M = -INFINITY, l = 0.f, o = 0.f;
-        for (int w = 0; w < NW; w++) M = fmaxf(M, recs[w * REC + h]);
-        for (int w = 0; w < NW; w++) {
-            const float m = recs[w * REC + h];
-            const float f = m == -INFINITY ? 0.f : fast_exp2(m - M);
-            l = fmaf(f, recs[w * REC + GMAX + h], l);
-            o = fmaf(f, recs[w * REC + 2 * GMAX + i], o);
+    const int W = pre[B];
+    for (int s = c; s < B; s += gridDim.x) {  // takes that hold nothing
+        if (Ls[s] > 0) continue;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < P.nq * HD / 8; i += NT)
+            reinterpret_cast<uint4 *>(P.out + static_cast<long>(s) * P.nq * HD)[i] = zero;
+        if (FUSED && P.held)
+            for (int i = threadIdx.x; i < 2 * nk * HD / 8; i += NT)
+                reinterpret_cast<uint4 *>(P.held + static_cast<long>(s) * 2 * nk * HD)[i] = zero;
+    }
+    const int want = (W + MIN_TILES - 1) / MIN_TILES, Gc = want < static_cast<int>(gridDim.x) ? want : gridDim.x;
+    if (c >= Gc) return;
+    const int ta = cut(c, Gc, W), tb = cut(c + 1, Gc, W);
+    const int wa = ta + cut(warp, NW, tb - ta), wb = ta + cut(warp + 1, NW, tb - ta), n = wb - wa;
+
+    // ---- this warp's tiles ----
+    if (n > 0) {
+        const uint8_t *src = nullptr;  // lane i: tile base + i
+        auto look_up = [&](int base) {
+            const int t = wa + base + lane;
+            if (t >= wb) return;
+            const int s = take_of(pre, B, t), T = tiles_of(Ls[s]), off = t - pre[s], kh = off / T, j = off - kh * T;
+            int page = P.table[static_cast<long>(s) * P.maxpages + j / 2];
+            if (page < 0 || page >= P.npages) {
+                record_error(OUMU_DEVERR_PAGE);
+                page = 0;  // read in its place: the take's output is unspecified
+            }
+            src = P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + (j & 1) * F::HALFB;
+        };
+        auto issue = [&](int k) {  // tile k into its stage
+            const unsigned long long a = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k & 31);
+            if (lane == 0) {
+                const uint32_t bar = bars + 8 * (k % ST);
+                mbar_expect_tx(bar, F::HALFB);
+                bulk_load(ring + (k % ST) * F::HALFB, reinterpret_cast<const void *>(a), F::HALFB, bar);
+            }
+        };
+        look_up(0);
+        for (int k = 0; k < ST && k < n; k++) issue(k);
+        int s = take_of(pre, B, wa), T = tiles_of(Ls[s]), kh = (wa - pre[s]) / T, j = wa - pre[s] - kh * T;
+        if (lane == 0) segs[warp] = make_int2(s * nk + kh, wa - j);
+        Query<HD> Q;
+        State<HD> S;
+        Newest<HD> N;
+        bool ok = true, fresh = true;
+        int issued = n < ST ? n : ST;
+        for (int k = 0; k < n; k++) {
+            const int L = Ls[s];
+            if (fresh) {
+                Q.load(P, s, kh, L - 1, lane);
+                S.clear();
+                if (FUSED && T - 1 - j < n - k) {  // the segment's last tile is this warp's
+                    const int page = P.table[static_cast<long>(s) * P.maxpages + (T - 1) / 2];
+                    if (page >= 0 && page < P.npages)
+                        N.make(P, s, kh, L - 1, lane,
+                               P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + ((T - 1) & 1) * F::HALFB);
+                }
+                fresh = false;
+            }
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(bars + 8 * (k % ST), (k / ST) & 1));
+            if (ok) {
+                uint8_t *half = sm + warp * Y::RING + (k % ST) * F::HALFB;
+                if (FUSED && j == T - 1) {
+                    N.patch(half, (L - 1) % HALF, lane);
+                    fence_proxy_async_smem();  // before the stage's next copy
+                    __syncwarp();
+                }
+                S.tile(half, L - j * HALF, Q, lane);
+            }
+            __syncwarp();
+            if (k + ST < n) {
+                if (((k + ST) & 31) == 0) look_up(k + ST);
+                if (ok) {
+                    issue(k + ST);
+                    issued++;
+                }
+            }
+            if (j == T - 1 || k == n - 1) {
+                // ---- the segment's end, or this warp's ----
+                const int Sg = wa + k - j;
+                if (Sg >= wa && j == T - 1) {
+                    S.finish(P.out + (static_cast<long>(s) * P.nq + kh * G) * HD, G, lane);
+                } else {
+                    float *R = k == n - 1 ? reinterpret_cast<float *>(sm + warp * Y::RING)
+                                          : reinterpret_cast<float *>(sm + Y::FIRST) + warp * Y::REC;
+                    S.record(R, lane);
+                }
+                fresh = true;
+            }
+            if (++j == T) {
+                j = 0;
+                if (++kh == nk) {
+                    kh = 0;
+                    do ++s; while (s < B && Ls[s] == 0);
+                    T = s < B ? tiles_of(Ls[s]) : 1;
+                }
+            }
         }
-        out[i] = f2bf(l > 0.f || l != l ? o / l : 0.f);
+        if (!ok)  // after a wait that ran out: no copy may still be on its way when the CTA leaves (bounded again)
+            for (int k = issued > ST ? issued - ST : 0; k < issued; k++) mbar_wait(bars + 8 * (k % ST), (k / ST) & 1);
+    }
+    __syncthreads();
+
+    // ---- segments that cross a boundary between warps, or the CTA's ends ----
+    constexpr int LPH = HD / 4;  // threads per head, 4 channels each
+    const int h = threadIdx.x / LPH, d4 = threadIdx.x % LPH;
+    int prev = -1;
+    for (int b = 0; b <= NW; b++) {
+        const int xb = ta + cut(b, NW, tb - ta);
+        if (b < NW && xb == ta + cut(b + 1, NW, tb - ta)) continue;  // a warp without tiles
+        int id, Sg;
+        if (b < NW) {
+            id = segs[b].x;
+            Sg = segs[b].y;
+            if (Sg >= xb) continue;
+        } else {
+            const int s = take_of(pre, B, tb - 1), T = tiles_of(Ls[s]), kh = (tb - 1 - pre[s]) / T;
+            id = s * nk + kh;
+            Sg = pre[s] + kh * T;
+            if (Sg + T <= tb) continue;
+        }
+        if (id == prev) continue;
+        prev = id;
+        const int s = id / nk, kh = id % nk, Eg = Sg + tiles_of(Ls[s]);
+        float M = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (h < G) {
+            for (int pass = 0; pass < 2; pass++)
+#pragma unroll
+                for (int w = 0; w < NW; w++) {
+                    const int a = ta + cut(w, NW, tb - ta), e = ta + cut(w + 1, NW, tb - ta);
+                    if (a == e || e <= Sg || a >= Eg) continue;
+                    const float *R = Eg >= e ? reinterpret_cast<const float *>(sm + w * Y::RING)
+                                             : reinterpret_cast<const float *>(sm + Y::FIRST) + w * Y::REC;
+                    if (pass == 0) {
+                        M = fmaxf(M, R[h]);
+                    } else {
+                        const float f = fast_exp2(R[h] - M);
+                        const float4 x = *reinterpret_cast<const float4 *>(R + 2 * GMAX + h * HD + 4 * d4);
+                        l = fmaf(f, R[GMAX + h], l);
+                        o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
+                    }
+                }
+        }
+        if (Sg < ta || Eg > tb) {
+            // tiles of it lie in other CTAs: cf .. cl. Record 1 of a CTA is of a segment that starts in it.
+            const int cf = static_cast<int>((static_cast<long>(Sg + 1) * Gc + W - 1) / W) - 1;
+            const int cl = static_cast<int>((static_cast<long>(Eg) * Gc + W - 1) / W) - 1;
+            float *rec = P.part + (static_cast<long>(c) * 2 + (c == cf)) * Y::REC;
+            if (h < G) {
+                if (d4 == 0) {
+                    rec[h] = M;
+                    rec[GMAX + h] = l;
+                }
+                *reinterpret_cast<float4 *>(rec + 2 * GMAX + h * HD + 4 * d4) = o;
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) misc[NW] = atomic_add_acq_rel(P.cnt + id, 1);
+            __syncthreads();
+            const bool last = misc[NW] == cl - cf;
+            __syncthreads();
+            if (!last) continue;
+            if (threadIdx.x == 0) P.cnt[id] = 0;
+            if (h < G) {
+                auto at = [&](int cc) { return P.part + (static_cast<long>(cc) * 2 + (cc == cf)) * Y::REC; };
+                M = -INFINITY;
+                for (int cc = cf; cc <= cl; cc++) M = fmaxf(M, __ldcg(at(cc) + h));
+                l = 0.f;
+                o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                for (int cc = cf; cc <= cl; cc++) {
+                    const float *R = at(cc);
+                    const float f = fast_exp2(__ldcg(R + h) - M);
+                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(R + 2 * GMAX + h * HD + 4 * d4));
+                    l = fmaf(f, __ldcg(R + GMAX + h), l);
+                    o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
+                }
+            }
+        }
+        if (h < G) {
+            const float r = 1.f / l;
+            uint2 u;
+            u.x = pack_bf16x2(o.x * r, o.y * r);
+            u.y = pack_bf16x2(o.z * r, o.w * r);
+            *reinterpret_cast<uint2 *>(P.out + (static_cast<long>(s) * P.nq + kh * G + h) * HD + 4 * d4) = u;
+        }
     }
 }
 

@@ -136,6 +136,9 @@ int current_device(int *sms) {
                                      kSmemMax));
         OUMU_CK(cudaFuncSetAttribute(gm::k_gemm<128, kGemmStages128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      kSmemMax));
+        for (auto kern : {d4::k_attn_decode_kv4<128, false>, d4::k_attn_decode_kv4<128, true>,
+                          d4::k_attn_decode_kv4<64, false>, d4::k_attn_decode_kv4<64, true>})
+            OUMU_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
         di.ready = true;
     }
     *sms = di.sms;
@@ -933,10 +936,11 @@ unsigned kv4_grid(int B, long blocks, int nk) {
 size_t kv4_part_bytes(int hd) { return 2 * (2 * static_cast<size_t>(d4::GMAX) + d4::GMAX * hd) * 4; }
 
 template <int HD, bool FUSED>
-int launch_decode_kv4(const d4::Params &P, cudaStream_t st) {
-    const int smem = d4::NW * (2 * d4::GMAX + d4::GMAX * HD) * 4;
-    OUMU_CK(launch_k(d4::k_attn_decode_kv4<HD, FUSED>, dim3(static_cast<unsigned>(P.B * P.nk)), dim3(d4::NW * 32), smem,
-                     st, P));
+int launch_decode_kv4(const d4::Params &P, size_t ws_bytes, int sms, cudaStream_t st) {
+    // one CTA per SM, fewer where the workspace holds fewer CTAs' records
+    const long fit = static_cast<long>((ws_bytes - decode_counter_bytes(P.B, P.nk)) / kv4_part_bytes(HD));
+    const unsigned grid = static_cast<unsigned>(std::min(static_cast<long>(sms), fit));
+    OUMU_CK(launch_k(d4::k_attn_decode_kv4<HD, FUSED>, dim3(grid), dim3(d4::NT), d4::Lay<HD>::bytes(P.B), st, P));
     return OUMU_OK;
 }
 
@@ -977,8 +981,11 @@ int decode_kv4_entry(bool fused, const void *qkv, void *pool, void *out, void *h
     P.maxpages = maxpages;
     P.sl2 = scale * 1.4426950408889634f;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (fused) return hd == 128 ? launch_decode_kv4<128, true>(P, st) : launch_decode_kv4<64, true>(P, st);
-    return hd == 128 ? launch_decode_kv4<128, false>(P, st) : launch_decode_kv4<64, false>(P, st);
+    if (fused)
+        return hd == 128 ? launch_decode_kv4<128, true>(P, ws_bytes, sms, st)
+                         : launch_decode_kv4<64, true>(P, ws_bytes, sms, st);
+    return hd == 128 ? launch_decode_kv4<128, false>(P, ws_bytes, sms, st)
+                     : launch_decode_kv4<64, false>(P, ws_bytes, sms, st);
 }
 
 // Pools of `layers` layers; layer_stride only matters from the second on.
