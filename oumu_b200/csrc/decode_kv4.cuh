@@ -26,13 +26,40 @@ using kv4::Words;
 constexpr int GMAX = 8;      // q heads per kv head handled by one mma column block
 constexpr float SMIN = 8.6736174e-19f;  // 2^-60: groups of smaller scale count as this when M is set
 
-__device__ __forceinline__ void mma_f16(float *d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+// Not volatile (nor the transposition below): the compiler may interleave these with other work as it likes.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = a * b, with nothing added
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     uint32_t r;
@@ -42,9 +69,19 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 // 8 codes of a word as fp16 pairs: n 2^-24 (even nibbles) and 16 n 2^-24 (odd ones)
 __device__ __forceinline__ uint32_t code_even(uint32_t w) { return w & 0x000f000fu; }
 __device__ __forceinline__ uint32_t code_odd(uint32_t w) { return w & 0x00f000f0u; }
-// The same with the high halves (V: the odd positions) as n - 15
-__device__ __forceinline__ uint32_t flip_even(uint32_t w) { return (w & 0x000f000fu) ^ 0x800f0000u; }
-__device__ __forceinline__ uint32_t flip_odd(uint32_t w) { return (w & 0x00f000f0u) ^ 0x80f00000u; }
+// The same with the high halves (V: the odd positions) as n - 15: (w & mask) ^ flip in one instruction
+__device__ __forceinline__ uint32_t and_xor(uint32_t w, uint32_t mask, uint32_t flip) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(w), "r"(mask), "r"(flip));
+    return r;
+}
+__device__ __forceinline__ uint32_t flip_even(uint32_t w) { return and_xor(w, 0x000f000fu, 0x800f0000u); }
+__device__ __forceinline__ uint32_t flip_odd(uint32_t w) { return and_xor(w, 0x00f000f0u, 0x80f00000u); }
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 
 struct Params {
     const bf16 *qkv;
@@ -154,73 +191,84 @@ struct Query {
     }
 };
 
-// The running state of one (take, kv head): lane 4g + t holds heads 2t and 2t + 1.
+// The running state of one (take, kv head): lane 4g + t holds heads 2t and 2t + 1. What goes with the codes beside them,
+// the zeros' term and the sum of p: for hd 128 by the matrix instructions too, the meta rows of 8 positions being an 8 x 8
+// matrix whose transpose (ldmatrix) is their operand, p in two bf16 parts (17 bits); for hd 64 by each lane for its
+// positions.
 template <int HD>
 struct State {
     static constexpr int W = Fmt<HD>::W;
-    float M[2], l[2];          // reference exponent; this lane's positions' share of the sum
+    static constexpr bool SIDE = W == 4;
+    float M[2];                // reference exponent
     float acc[2 * W][4];       // numerator / 2^24 of channels 32w + 4g + {0 | 1 (x 16)}, {2 | 3 (x 16)}
-    float z[W][2];             // this lane's positions' share of the zeros' term
+    // SIDE: [0..1] row g: sum p s_g (g < 4, not used) | sum p z of group g - 4; [2..3] row 8 + g: sum over odd positions
+    // of p s_g (g < 4) | sum p. Otherwise: [2w + c] this lane's share of the zeros' term, [2W + c] of the sum.
+    float side[SIDE ? 4 : 2 * W + 2];
     __device__ void clear() {
         M[0] = M[1] = -INFINITY;
-        l[0] = l[1] = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * W; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; w++) z[w][0] = z[w][1] = 0.f;
+        for (float &f : side) f = 0.f;
     }
 
-    // One tile of 32 positions at `half`, the first `n` of them valid (what lies behind is never used: its codes are
-    // finite whatever they hold, its scales and zeros are replaced).
-    __device__ __forceinline__ void tile(const uint8_t *half, int n, const Query<HD> &Q, int lane) {
+    // One tile of 32 positions in shared memory, the first `n` of them valid (what lies behind is never used: its codes
+    // are finite whatever they hold, the scales and zeros of its V are cleared here).
+    __device__ __forceinline__ void tile(uint8_t *half, int n, const Query<HD> &Q, int lane) {
         using F = Fmt<HD>;
         const int g = lane >> 2, t = lane & 3;
-        const float c15 = g & 1 ? 15.f : 0.f;
         float x[2][4];
+        {
+            // the instructions of all groups and halves side by side: two dependent ones a group, 2 W independent chains
+            Words<W> k[2][2], m[2][2];
+            float a[2][W][4];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const Words<W> k0 = kv4::ld_words<W>(half + (2 * h) * F::BLOCK + lane * 4 * W);
-            const Words<W> k1 = kv4::ld_words<W>(half + (2 * h + 1) * F::BLOCK + lane * 4 * W);
-            const Words<W> m0 = kv4::ld_words<W>(half + F::KMETA + (16 * h + g) * F::ROW);
-            const Words<W> m1 = kv4::ld_words<W>(half + F::KMETA + (16 * h + 8 + g) * F::ROW);
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            const uint32_t a0 = W == 4 ? (t & 1 ? m0.v[W - 1] : m0.v[W / 2]) : m0.v[W - 1];
-            const uint32_t a1 = W == 4 ? (t & 1 ? m1.v[W - 1] : m1.v[W / 2]) : m1.v[W - 1];
-            mma_bf16_16816(d, a0, a1, a0, a1, Q.z0, Q.z1);
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int w = 0; w < W; w++) {
-                float a[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16(a, code_even(k0.v[w]), code_even(k1.v[w]), code_odd(k0.v[w]), code_odd(k1.v[w]), Q.q[w][0],
-                        Q.q[w][1]);
-                mma_f16(a, code_even(k0.v[w] >> 8), code_even(k1.v[w] >> 8), code_odd(k0.v[w] >> 8),
-                        code_odd(k1.v[w] >> 8), Q.q[w][2], Q.q[w][3]);
-                const float s0 = kv4::row_scale<W>(m0, w), s1 = kv4::row_scale<W>(m1, w);
-                d[0] = fmaf(s0, a[0], d[0]);
-                d[1] = fmaf(s0, a[1], d[1]);
-                d[2] = fmaf(s1, a[2], d[2]);
-                d[3] = fmaf(s1, a[3], d[3]);
+                for (int r = 0; r < 2; r++) {
+                    k[h][r] = kv4::ld_words<W>(half + (2 * h + r) * F::BLOCK + lane * 4 * W);
+                    m[h][r] = kv4::ld_words<W>(half + F::KMETA + (16 * h + 8 * r + g) * F::ROW);
+                }
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int w = 0; w < W; w++)
+                    mma_f16_new(a[h][w], code_even(k[h][0].v[w]), code_even(k[h][1].v[w]), code_odd(k[h][0].v[w]),
+                                code_odd(k[h][1].v[w]), Q.q[w][0], Q.q[w][1]);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t a0 = W == 4 && !(t & 1) ? m[h][0].v[W / 2] : m[h][0].v[W - 1];
+                const uint32_t a1 = W == 4 && !(t & 1) ? m[h][1].v[W / 2] : m[h][1].v[W - 1];
+                mma_bf16_new(x[h], a0, a1, a0, a1, Q.z0, Q.z1);
             }
-            x[h][0] = d[0] * Q.mul0;
-            x[h][1] = d[1] * Q.mul1;
-            x[h][2] = d[2] * Q.mul0;
-            x[h][3] = d[3] * Q.mul1;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int w = 0; w < W; w++)
+                    mma_f16(a[h][w], code_even(k[h][0].v[w] >> 8), code_even(k[h][1].v[w] >> 8),
+                            code_odd(k[h][0].v[w] >> 8), code_odd(k[h][1].v[w] >> 8), Q.q[w][2], Q.q[w][3]);
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int w = 0; w < W; w++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[h][i] = fmaf(kv4::row_scale<W>(m[h][i >> 1], w), a[h][w][i], x[h][i]);
+        }
+        if (n < HALF) {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (16 * h + 8 * (i >> 1) + g >= n) x[h][i] = -INFINITY;
+            if (lane >= n) kv4::st_words<W>(half + F::VMETA + lane * F::ROW, Words<W>{});
+            fence_proxy_async_smem();  // before the stage's next copy
+            __syncwarp();
         }
         Words<W> vm[2][2];
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int r = 0; r < 2; r++) vm[h][r] = kv4::ld_words<W>(half + F::VMETA + (16 * h + 8 * r + g) * F::ROW);
-        if (n < HALF) {
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int r = 0; r < 2; r++)
-                    if (16 * h + 8 * r + g >= n) {
-                        x[h][2 * r] = x[h][2 * r + 1] = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < W; i++) vm[h][r].v[i] = 0u;
-                    }
-        }
         float p[2][4];
         uint32_t pv[2][W][2];
         auto weights = [&]() -> bool {  // p and p s; true where M is too low for them
@@ -229,39 +277,65 @@ struct State {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    p[h][i] = fast_exp2(x[h][i] - M[i & 1]);
-                    big = fmaxf(big, p[h][i]);
-                }
+                for (int i = 0; i < 4; i++) p[h][i] = fast_exp2(fmaf(x[h][i], i & 1 ? Q.mul1 : Q.mul0, -M[i & 1]));
+                big = fmax3(fmax3(big, p[h][0], p[h][1]), p[h][2], p[h][3]);
 #pragma unroll
                 for (int w = 0; w < W; w++)
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
                         const float s = kv4::row_scale<W>(vm[h][r], w);
                         pv[h][w][r] = pack_f16x2(p[h][2 * r] * s, p[h][2 * r + 1] * s);
-                        top = __vmaxu2(top, pv[h][w][r]);
+                        top = max_u16x2(top, pv[h][w][r]);
                     }
             }
             // 2^15 in fp16 is 0x7800 (infinities and NaN lie above); p itself may reach 2^75 where every scale is tiny
-            return (top & 0xffffu) > 0x7800u || top >> 16 > 0x7800u || !(big <= 3.7778932e22f);
+            return (top & 0xffffu) > 0x7800u || top > 0x7800ffffu || !(big <= 3.7778932e22f);
         };
         if (__any_sync(0xffffffffu, weights())) {
-            rescale(x, vm, lane);
+            rescale(x, vm, Q);
             weights();
+        }
+        if constexpr (SIDE) {
+            uint32_t r[4];
+            ldsm_x4_t(smem_u32(half + F::VMETA + lane * F::ROW), r[0], r[1], r[2], r[3]);
+            const uint32_t keep = g < 4 ? 0xffff0000u : 0u, one = g < 4 ? 0u : 0x3f803f80u;
+            float d[4];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t u0 = pack_bf16x2(p[h][0], p[h][1]), u1 = pack_bf16x2(p[h][2], p[h][3]);
+                const float2 f0 = unpack_bf16x2(u0), f1 = unpack_bf16x2(u1);
+                const uint32_t v0 = pack_bf16x2(p[h][0] - f0.x, p[h][1] - f0.y);
+                const uint32_t v1 = pack_bf16x2(p[h][2] - f1.x, p[h][3] - f1.y);
+                const uint32_t a0 = r[2 * h], a2 = r[2 * h + 1], a1 = (a0 & keep) | one, a3 = (a2 & keep) | one;
+                if (h == 0) mma_bf16_new(d, a0, a1, a2, a3, transpose8(u0), transpose8(u1));
+                else mma_bf16(d, a0, a1, a2, a3, transpose8(u0), transpose8(u1));
+                mma_bf16(d, a0, a1, a2, a3, transpose8(v0), transpose8(v1));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) side[i] += d[i];  // rounded, not cut: these sums keep one sign
+        } else {
+            const float c15 = g & 1 ? 15.f : 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    side[2 * W + c] += p[h][c] + p[h][2 + c];
+#pragma unroll
+                    for (int w = 0; w < W; w++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++)
+                            side[2 * w + c] = fmaf(
+                                p[h][2 * r + c],
+                                fmaf(c15, kv4::row_scale<W>(vm[h][r], w), kv4::row_zero<W>(vm[h][r], w)), side[2 * w + c]);
+                }
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            l[0] += p[h][0] + p[h][2];
-            l[1] += p[h][1] + p[h][3];
             const Words<W> v0 = kv4::ld_words<W>(half + F::CODES + (2 * h) * F::BLOCK + lane * 4 * W);
             const Words<W> v1 = kv4::ld_words<W>(half + F::CODES + (2 * h + 1) * F::BLOCK + lane * 4 * W);
 #pragma unroll
             for (int w = 0; w < W; w++) {
-                const float z0 = fmaf(c15, kv4::row_scale<W>(vm[h][0], w), kv4::row_zero<W>(vm[h][0], w));
-                const float z1 = fmaf(c15, kv4::row_scale<W>(vm[h][1], w), kv4::row_zero<W>(vm[h][1], w));
-                z[w][0] = fmaf(p[h][0], z0, fmaf(p[h][2], z1, z[w][0]));
-                z[w][1] = fmaf(p[h][1], z0, fmaf(p[h][3], z1, z[w][1]));
-                const uint32_t b0 = movmatrix_t(pv[h][w][0]), b1 = movmatrix_t(pv[h][w][1]);
+                const uint32_t b0 = transpose8(pv[h][w][0]), b1 = transpose8(pv[h][w][1]);
                 mma_f16(acc[2 * w], flip_even(v0.v[w]), flip_odd(v0.v[w]), flip_even(v1.v[w]), flip_odd(v1.v[w]), b0,
                         b1);
                 mma_f16(acc[2 * w + 1], flip_even(v0.v[w] >> 8), flip_odd(v0.v[w] >> 8), flip_even(v1.v[w] >> 8),
@@ -272,7 +346,7 @@ struct State {
 
     // Raise M so that the largest p s of this tile is 2^10, and bring the sums along. The first tile of a state always
     // comes here (M = -inf); later ones when a logit rises by more than 5 over everything before.
-    __device__ __forceinline__ void rescale(const float (&x)[2][4], const Words<W> (&vm)[2][2], int lane) {
+    __device__ __forceinline__ void rescale(const float (&x)[2][4], const Words<W> (&vm)[2][2], const Query<HD> &Q) {
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int h = 0; h < 2; h++)
@@ -282,8 +356,8 @@ struct State {
 #pragma unroll
                 for (int w = 0; w < W; w++) s = fmaxf(s, kv4::row_scale<W>(vm[h][r], w));
                 const float ls = __log2f(s);
-                top[0] = fmaxf(top[0], x[h][2 * r] + ls);
-                top[1] = fmaxf(top[1], x[h][2 * r + 1] + ls);
+                top[0] = fmaxf(top[0], fmaf(x[h][2 * r], Q.mul0, ls));
+                top[1] = fmaxf(top[1], fmaf(x[h][2 * r + 1], Q.mul1, ls));
             }
 #pragma unroll
         for (int c = 0; c < 2; c++) {
@@ -293,30 +367,42 @@ struct State {
             if (m == -INFINITY) m = 0.f;
             const float f = fast_exp2(M[c] - m);
             M[c] = m;
-            l[c] *= f;
 #pragma unroll
             for (int i = 0; i < 2 * W; i++) {
                 acc[i][c] *= f;
                 acc[i][c + 2] *= f;
             }
 #pragma unroll
-            for (int w = 0; w < W; w++) z[w][c] *= f;
+            for (int i = c; i < (SIDE ? 4 : 2 * W + 2); i += 2) side[i] *= f;
         }
     }
 
-    // The lanes' shares of the sum and of the zeros' term, added up over the positions.
-    __device__ __forceinline__ void reduce() {
+    // The sums of p and the zeros' terms of heads 2t and 2t + 1 over all positions, in every lane.
+    __device__ __forceinline__ void reduce(float (&l)[2], float (&z)[W][2], int lane) const {
 #pragma unroll
-        for (int c = 0; c < 2; c++)
+        for (int c = 0; c < 2; c++) {
+            if constexpr (SIDE) {
+                const int t = lane & 3;
+                l[c] = __shfl_sync(0xffffffffu, side[2 + c], 16 + t);
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                l[c] += __shfl_xor_sync(0xffffffffu, l[c], o);
+                for (int w = 0; w < W; w++)
+                    z[w][c] = fmaf(15.f, __shfl_sync(0xffffffffu, side[2 + c], 4 * w + t),
+                                   __shfl_sync(0xffffffffu, side[c], 16 + 4 * w + t));
+            } else {
+                l[c] = side[2 * W + c];
 #pragma unroll
-                for (int w = 0; w < W; w++) z[w][c] += __shfl_xor_sync(0xffffffffu, z[w][c], o);
+                for (int w = 0; w < W; w++) z[w][c] = side[2 * w + c];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    l[c] += __shfl_xor_sync(0xffffffffu, l[c], o);
+#pragma unroll
+                    for (int w = 0; w < W; w++) z[w][c] += __shfl_xor_sync(0xffffffffu, z[w][c], o);
+                }
             }
+        }
     }
     // Numerators of head 2t + c, channels 32w + 4g .. + 3, with the zeros' term, in the values' own unit.
-    __device__ __forceinline__ float4 numerators(int w, int c) const {
+    __device__ __forceinline__ float4 numerators(const float (&z)[W][2], int w, int c) const {
         const float u = 16777216.f, u16 = 1048576.f;  // 2^24, and / 16 for the odd nibbles
         return make_float4(fmaf(acc[2 * w][c], u, z[w][c]), fmaf(acc[2 * w][c + 2], u16, z[w][c]),
                            fmaf(acc[2 * w + 1][c], u, z[w][c]), fmaf(acc[2 * w + 1][c + 2], u16, z[w][c]));
@@ -324,14 +410,15 @@ struct State {
     // The output of a segment that this warp has seen whole; out: its first head's row.
     __device__ __forceinline__ void finish(bf16 *out, int G, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        reduce();
+        float l[2], z[W][2];
+        reduce(l, z, lane);
 #pragma unroll
         for (int c = 0; c < 2; c++) {
             if (2 * t + c >= G) continue;
             const float r = 1.f / l[c];
 #pragma unroll
             for (int w = 0; w < W; w++) {
-                const float4 o = numerators(w, c);
+                const float4 o = numerators(z, w, c);
                 uint2 u;
                 u.x = pack_bf16x2(o.x * r, o.y * r);
                 u.y = pack_bf16x2(o.z * r, o.w * r);
@@ -342,7 +429,8 @@ struct State {
     // The state as a record: m[8], l[8], o[8][HD].
     __device__ __forceinline__ void record(float *R, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        reduce();
+        float l[2], z[W][2];
+        reduce(l, z, lane);
         if (g == 0) {
             R[2 * t] = M[0];
             R[2 * t + 1] = M[1];
@@ -353,7 +441,7 @@ struct State {
         for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int w = 0; w < W; w++)
-                *reinterpret_cast<float4 *>(R + 2 * GMAX + (2 * t + c) * HD + 32 * w + 4 * g) = numerators(w, c);
+                *reinterpret_cast<float4 *>(R + 2 * GMAX + (2 * t + c) * HD + 32 * w + 4 * g) = numerators(z, w, c);
     }
 };
 
@@ -456,7 +544,7 @@ struct Lay {
     static constexpr int BAR = FIRST + NW * REC * 4;
     static constexpr int SEG = BAR + NW * ST * 8;     // first segment of each warp: id, start
     static constexpr int MISC = SEG + NW * 8;
-    static constexpr int PRE = MISC + 64;             // pre[B + 1], lens[B]
+    static constexpr int PRE = MISC + 128;            // pre[B + 1], lens[B]
     static __host__ __device__ int bytes(int B) { return PRE + (2 * B + 1) * 4; }
 };
 
@@ -487,9 +575,16 @@ __device__ __forceinline__ int take_of(const int *pre, int B, int t) {
     }
     return lo;
 }
-__device__ __forceinline__ int cut(int i, int n, int W) {  // start of part i of W tiles in n parts
-    return static_cast<int>(static_cast<long>(i) * W / n);
-}
+// W tiles in n parts, the first W % n of them one tile longer: where part i starts, and the part that has tile t.
+struct Parts {
+    int q, r;
+    __device__ Parts(int W, int n) : q(W / n), r(W % n) {}
+    __device__ int start(int i) const { return i * q + min(i, r); }
+    __device__ int of(int t) const {
+        const int a = r * (q + 1);
+        return t < a ? t / (q + 1) : r + (t - a) / q;
+    }
+};
 
 template <int HD, bool FUSED>
 __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
@@ -548,8 +643,10 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
     }
     const int want = (W + MIN_TILES - 1) / MIN_TILES, Gc = want < static_cast<int>(gridDim.x) ? want : gridDim.x;
     if (c >= Gc) return;
-    const int ta = cut(c, Gc, W), tb = cut(c + 1, Gc, W);
-    const int wa = ta + cut(warp, NW, tb - ta), wb = ta + cut(warp + 1, NW, tb - ta), n = wb - wa;
+    const Parts ctas(W, Gc);
+    const int ta = ctas.start(c), tb = ctas.start(c + 1);
+    const Parts parts(tb - ta, NW);
+    const int wa = ta + parts.start(warp), wb = ta + parts.start(warp + 1), n = wb - wa;
 
     // ---- this warp's tiles ----
     if (n > 0) {
@@ -595,7 +692,9 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
                 }
                 fresh = false;
             }
-            ok = __all_sync(0xffffffffu, ok && mbar_wait(bars + 8 * (k % ST), (k / ST) & 1));
+            const uint32_t bar = bars + 8 * (k % ST), phase = (k / ST) & 1;
+            if (!__all_sync(0xffffffffu, ok && mbar_try_wait(bar, phase)))
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, phase));
             if (ok) {
                 uint8_t *half = sm + warp * Y::RING + (k % ST) * F::HALFB;
                 if (FUSED && j == T - 1) {
@@ -644,8 +743,8 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
     const int h = threadIdx.x / LPH, d4 = threadIdx.x % LPH;
     int prev = -1;
     for (int b = 0; b <= NW; b++) {
-        const int xb = ta + cut(b, NW, tb - ta);
-        if (b < NW && xb == ta + cut(b + 1, NW, tb - ta)) continue;  // a warp without tiles
+        const int xb = ta + parts.start(b);
+        if (b < NW && xb == tb) continue;  // a warp without tiles
         int id, Sg;
         if (b < NW) {
             id = segs[b].x;
@@ -666,7 +765,7 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
             for (int pass = 0; pass < 2; pass++)
 #pragma unroll
                 for (int w = 0; w < NW; w++) {
-                    const int a = ta + cut(w, NW, tb - ta), e = ta + cut(w + 1, NW, tb - ta);
+                    const int a = ta + parts.start(w), e = ta + parts.start(w + 1);
                     if (a == e || e <= Sg || a >= Eg) continue;
                     const float *R = Eg >= e ? reinterpret_cast<const float *>(sm + w * Y::RING)
                                              : reinterpret_cast<const float *>(sm + Y::FIRST) + w * Y::REC;
@@ -682,8 +781,7 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
         }
         if (Sg < ta || Eg > tb) {
             // tiles of it lie in other CTAs: cf .. cl. Record 1 of a CTA is of a segment that starts in it.
-            const int cf = static_cast<int>((static_cast<long>(Sg + 1) * Gc + W - 1) / W) - 1;
-            const int cl = static_cast<int>((static_cast<long>(Eg) * Gc + W - 1) / W) - 1;
+            const int cf = ctas.of(Sg), cl = ctas.of(Eg - 1);
             float *rec = P.part + (static_cast<long>(c) * 2 + (c == cf)) * Y::REC;
             if (h < G) {
                 if (d4 == 0) {
