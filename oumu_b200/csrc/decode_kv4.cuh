@@ -535,6 +535,11 @@ constexpr int ST = 4;           // tiles in flight per warp: 8 x 4 x 5 KB = 160 
 constexpr int NT = NW * 32;
 constexpr int MIN_TILES = 2 * NW;  // tiles per CTA at least
 
+// A segment that crosses a boundary: take * nk + kv head, its tiles, the CTA's warps that have some of them.
+struct Cross {
+    int id, start, end, first, last;
+};
+
 template <int HD>
 struct Lay {
     static constexpr int REC = 2 * GMAX + GMAX * HD;  // floats of a record: m[8], l[8], o[8][HD]
@@ -542,8 +547,8 @@ struct Lay {
     static constexpr int RING = ST * Fmt<HD>::HALFB;
     static constexpr int FIRST = NW * RING;           // records of segments that end inside a warp's range
     static constexpr int BAR = FIRST + NW * REC * 4;
-    static constexpr int SEG = BAR + NW * ST * 8;     // first segment of each warp: id, start
-    static constexpr int MISC = SEG + NW * 8;
+    static constexpr int LIST = BAR + NW * ST * 8;    // segments that cross warps
+    static constexpr int MISC = LIST + (NW + 1) * static_cast<int>(sizeof(Cross));
     static constexpr int PRE = MISC + 128;            // pre[B + 1], lens[B]
     static __host__ __device__ int bytes(int B) { return PRE + (2 * B + 1) * 4; }
 };
@@ -593,7 +598,6 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
     extern __shared__ __align__(128) uint8_t sm[];
     int *pre = reinterpret_cast<int *>(sm + Y::PRE), *Ls = pre + P.B + 1;
     int *misc = reinterpret_cast<int *>(sm + Y::MISC);
-    int2 *segs = reinterpret_cast<int2 *>(sm + Y::SEG);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int B = P.B, nk = P.nk, G = P.nq / P.nk, c = blockIdx.x;
     const uint32_t ring = smem_u32(sm) + warp * Y::RING, bars = smem_u32(sm) + Y::BAR + warp * ST * 8;
@@ -671,9 +675,8 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
             }
         };
         look_up(0);
-        for (int k = 0; k < ST && k < n; k++) issue(k);
+        issue(0);
         int s = take_of(pre, B, wa), T = tiles_of(Ls[s]), kh = (wa - pre[s]) / T, j = wa - pre[s] - kh * T;
-        if (lane == 0) segs[warp] = make_int2(s * nk + kh, wa - j);
         Query<HD> Q;
         State<HD> S;
         Newest<HD> N;
@@ -692,6 +695,8 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
                 }
                 fresh = false;
             }
+            if (k == 0)  // the first tile went ahead; the others follow behind every warp's first
+                for (int i = 1; i < ST && i < n; i++) issue(i);
             const uint32_t bar = bars + 8 * (k % ST), phase = (k / ST) & 1;
             if (!__all_sync(0xffffffffu, ok && mbar_try_wait(bar, phase)))
                 ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, phase));
@@ -739,87 +744,120 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
     __syncthreads();
 
     // ---- segments that cross a boundary between warps, or the CTA's ends ----
+    // Warp 0 lists them: boundary b (where warp b starts; b == NW: the CTA's end) lies inside one, unless it is the one
+    // before it again. The loops below are not unrolled: run once per launch, they cost their instruction fetches.
+    Cross *list = reinterpret_cast<Cross *>(sm + Y::LIST);
+    if (warp == 0) {
+        Cross x{-1, 0, 0, 0, 0};
+        const int at = ta + parts.start(lane < NW ? lane : NW);
+        const bool any = lane < NW ? at < tb : lane == NW;  // a warp without tiles starts where the CTA ends
+        if (any) {
+            // the segment of tile `at`, at the CTA's end of the tile before: its start is known to the warp that has it
+            const int s = take_of(pre, B, lane < NW ? at : tb - 1), T = tiles_of(Ls[s]);
+            const int kh = ((lane < NW ? at : tb - 1) - pre[s]) / T;
+            x.id = s * nk + kh;
+            x.start = pre[s] + kh * T;
+            x.end = x.start + T;
+            if (x.start >= at || x.end <= at) x.id = -1;  // starts here, or ends here
+        }
+        // the boundary before it, that of the last warp with tiles for the CTA's end
+        const int before = __shfl_sync(0xffffffffu, x.id, lane == NW ? min(NW, tb - ta) - 1 : lane - 1);
+        const unsigned in = __ballot_sync(0xffffffffu, x.id >= 0 && (lane == 0 || x.id != before));
+        if (in >> lane & 1) {
+            x.first = parts.of(max(x.start, ta) - ta);
+            x.last = parts.of(min(x.end, tb) - 1 - ta);
+            list[__popc(in & ((1u << lane) - 1))] = x;
+        }
+        if (lane == 0) misc[0] = __popc(in);
+    }
+    __syncthreads();
+    const int nlist = misc[0];
     constexpr int LPH = HD / 4;  // threads per head, 4 channels each
     const int h = threadIdx.x / LPH, d4 = threadIdx.x % LPH;
-    int prev = -1;
-    for (int b = 0; b <= NW; b++) {
-        const int xb = ta + parts.start(b);
-        if (b < NW && xb == tb) continue;  // a warp without tiles
-        int id, Sg;
-        if (b < NW) {
-            id = segs[b].x;
-            Sg = segs[b].y;
-            if (Sg >= xb) continue;
-        } else {
-            const int s = take_of(pre, B, tb - 1), T = tiles_of(Ls[s]), kh = (tb - 1 - pre[s]) / T;
-            id = s * nk + kh;
-            Sg = pre[s] + kh * T;
-            if (Sg + T <= tb) continue;
-        }
-        if (id == prev) continue;
-        prev = id;
-        const int s = id / nk, kh = id % nk, Eg = Sg + tiles_of(Ls[s]);
+    auto store = [&](int id, float l, float4 o) {
+        const float r = 1.f / l;
+        uint2 u;
+        u.x = pack_bf16x2(o.x * r, o.y * r);
+        u.y = pack_bf16x2(o.z * r, o.w * r);
+        *reinterpret_cast<uint2 *>(P.out + (static_cast<long>(id / nk) * P.nq + id % nk * G + h) * HD + 4 * d4) = u;
+    };
+    auto add = [&](float f, float lw, float4 x, float &l, float4 &o) {
+        l = fmaf(f, lw, l);
+        o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
+    };
+    int crossing = 0;  // entries that reach into other CTAs: the first, the last, or none
+#pragma unroll 1
+    for (int i = 0; i < nlist; i++) {
+        const Cross x = list[i];
+        const bool out = x.start < ta || x.end > tb;
+        crossing |= out << (i > 0 && i == nlist - 1);
+        if (h >= G) continue;
+        auto at = [&](int w) {  // warp w's record of it: its last one if the segment goes on to the range's end
+            return x.end >= ta + parts.start(w + 1) ? reinterpret_cast<const float *>(sm + w * Y::RING)
+                                                    : reinterpret_cast<const float *>(sm + Y::FIRST) + w * Y::REC;
+        };
         float M = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (h < G) {
-            for (int pass = 0; pass < 2; pass++)
+#pragma unroll 1
+        for (int w = x.first; w <= x.last; w++) M = fmaxf(M, at(w)[h]);
+#pragma unroll 1
+        for (int w = x.first; w <= x.last; w++) {
+            const float *R = at(w);
+            add(fast_exp2(R[h] - M), R[GMAX + h], *reinterpret_cast<const float4 *>(R + 2 * GMAX + h * HD + 4 * d4), l,
+                o);
+        }
+        if (!out) {
+            store(x.id, l, o);
+        } else {  // record 1 of a CTA is of a segment that starts in it
+            float *rec = P.part + (static_cast<long>(c) * 2 + (x.start >= ta)) * Y::REC;
+            if (d4 == 0) {
+                rec[h] = M;
+                rec[GMAX + h] = l;
+            }
+            *reinterpret_cast<float4 *>(rec + 2 * GMAX + h * HD + 4 * d4) = o;
+        }
+    }
+    if (!crossing) return;
+    // the counts of the (at most two) segments that reach into other CTAs; whoever completes one adds it up
+    __syncthreads();
+    if (threadIdx.x < 2 && crossing >> threadIdx.x & 1) {
+        const Cross x = list[threadIdx.x ? nlist - 1 : 0];
+        const int others = ctas.of(x.end - 1) - ctas.of(x.start);
+        const bool done = atomic_add_acq_rel(P.cnt + x.id, 1) == others;
+        if (done) P.cnt[x.id] = 0;
+        misc[1 + threadIdx.x] = done;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int k = 0; k < 2; k++) {
+        if (!(crossing >> k & 1) || !misc[1 + k] || h >= G) continue;
+        const Cross x = list[k ? nlist - 1 : 0];
+        const int cf = ctas.of(x.start), cl = ctas.of(x.end - 1);
+        auto at = [&](int cc) { return P.part + (static_cast<long>(cc) * 2 + (cc == cf)) * Y::REC; };
+        // the head's LPH threads take a record's reference each
+        float M = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int cc = cf + d4; cc <= cl; cc += LPH) M = fmaxf(M, __ldcg(at(cc) + h));
 #pragma unroll
-                for (int w = 0; w < NW; w++) {
-                    const int a = ta + parts.start(w), e = ta + parts.start(w + 1);
-                    if (a == e || e <= Sg || a >= Eg) continue;
-                    const float *R = Eg >= e ? reinterpret_cast<const float *>(sm + w * Y::RING)
-                                             : reinterpret_cast<const float *>(sm + Y::FIRST) + w * Y::REC;
-                    if (pass == 0) {
-                        M = fmaxf(M, R[h]);
-                    } else {
-                        const float f = fast_exp2(R[h] - M);
-                        const float4 x = *reinterpret_cast<const float4 *>(R + 2 * GMAX + h * HD + 4 * d4);
-                        l = fmaf(f, R[GMAX + h], l);
-                        o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
-                    }
-                }
-        }
-        if (Sg < ta || Eg > tb) {
-            // tiles of it lie in other CTAs: cf .. cl. Record 1 of a CTA is of a segment that starts in it.
-            const int cf = ctas.of(Sg), cl = ctas.of(Eg - 1);
-            float *rec = P.part + (static_cast<long>(c) * 2 + (c == cf)) * Y::REC;
-            if (h < G) {
-                if (d4 == 0) {
-                    rec[h] = M;
-                    rec[GMAX + h] = l;
-                }
-                *reinterpret_cast<float4 *>(rec + 2 * GMAX + h * HD + 4 * d4) = o;
+        for (int e = 1; e < LPH; e <<= 1)  // a head's threads come here together
+            M = fmaxf(M, __shfl_xor_sync(LPH == 32 ? 0xffffffffu : 0xffffu << (lane & 16), M, e, LPH));
+#pragma unroll 1
+        for (int c0 = cf; c0 <= cl; c0 += 8) {
+            float m[8], lw[8];
+            float4 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float *R = at(min(c0 + e, cl));
+                m[e] = __ldcg(R + h);
+                lw[e] = __ldcg(R + GMAX + h);
+                v[e] = __ldcg(reinterpret_cast<const float4 *>(R + 2 * GMAX + h * HD + 4 * d4));
             }
-            __syncthreads();
-            if (threadIdx.x == 0) misc[NW] = atomic_add_acq_rel(P.cnt + id, 1);
-            __syncthreads();
-            const bool last = misc[NW] == cl - cf;
-            __syncthreads();
-            if (!last) continue;
-            if (threadIdx.x == 0) P.cnt[id] = 0;
-            if (h < G) {
-                auto at = [&](int cc) { return P.part + (static_cast<long>(cc) * 2 + (cc == cf)) * Y::REC; };
-                M = -INFINITY;
-                for (int cc = cf; cc <= cl; cc++) M = fmaxf(M, __ldcg(at(cc) + h));
-                l = 0.f;
-                o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                for (int cc = cf; cc <= cl; cc++) {
-                    const float *R = at(cc);
-                    const float f = fast_exp2(__ldcg(R + h) - M);
-                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(R + 2 * GMAX + h * HD + 4 * d4));
-                    l = fmaf(f, __ldcg(R + GMAX + h), l);
-                    o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
-                }
-            }
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (c0 + e <= cl) add(fast_exp2(m[e] - M), lw[e], v[e], l, o);
         }
-        if (h < G) {
-            const float r = 1.f / l;
-            uint2 u;
-            u.x = pack_bf16x2(o.x * r, o.y * r);
-            u.y = pack_bf16x2(o.z * r, o.w * r);
-            *reinterpret_cast<uint2 *>(P.out + (static_cast<long>(s) * P.nq + kh * G + h) * HD + 4 * d4) = u;
-        }
+        store(x.id, l, o);
     }
 }
 
