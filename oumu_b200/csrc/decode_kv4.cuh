@@ -271,7 +271,8 @@ struct State {
             for (int r = 0; r < 2; r++) vm[h][r] = kv4::ld_words<W>(half + F::VMETA + (16 * h + 8 * r + g) * F::ROW);
         float p[2][4];
         uint32_t pv[2][W][2];
-        auto weights = [&]() -> bool {  // p and p s; true where M is too low for them
+        // p and p s, again where M turns out too low for them
+        for (bool again = false;; again = true) {
             uint32_t top = 0;
             float big = 0.f;
 #pragma unroll
@@ -289,11 +290,9 @@ struct State {
                     }
             }
             // 2^15 in fp16 is 0x7800 (infinities and NaN lie above); p itself may reach 2^75 where every scale is tiny
-            return (top & 0xffffu) > 0x7800u || top > 0x7800ffffu || !(big <= 3.7778932e22f);
-        };
-        if (__any_sync(0xffffffffu, weights())) {
+            const bool over = (top & 0xffffu) > 0x7800u || top > 0x7800ffffu || !(big <= 3.7778932e22f);
+            if (again || !__any_sync(0xffffffffu, over)) break;
             rescale(x, vm, Q);
-            weights();
         }
         if constexpr (SIDE) {
             uint32_t r[4];
@@ -533,6 +532,7 @@ struct Newest {
 constexpr int NW = 8;           // warps
 constexpr int ST = 4;           // tiles in flight per warp: 8 x 4 x 5 KB = 160 KB per SM
 constexpr int NT = NW * 32;
+static_assert(NW <= 16, "a half warp holds a reference per warp");
 constexpr int MIN_TILES = 2 * NW;  // tiles per CTA at least
 
 // A segment that crosses a boundary: take * nk + kv head, its tiles, the CTA's warps that have some of them.
@@ -553,10 +553,15 @@ struct Lay {
     static __host__ __device__ int bytes(int B) { return PRE + (2 * B + 1) * 4; }
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
+// The warp's first lane announces and starts a copy (predicated: no branch in the loop).
+__device__ __forceinline__ void bulk_load_first_lane(uint32_t dst, unsigned long long src, uint32_t bytes, uint32_t bar,
+                                                     int lane) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 st;\n setp.eq.s32 p, %4, 0;\n"
+        " @p mbarrier.arrive.expect_tx.shared::cta.b64 st, [%3], %2;\n"
+        " @p cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n}" ::"r"(dst),
+        "l"(src), "r"(bytes), "r"(bar), "r"(lane)
+        : "memory");
 }
 
 // Take s's length: lens[s] or *pos + 1, cut to what its table row can hold (recorded).
@@ -652,102 +657,10 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
     const Parts parts(tb - ta, NW);
     const int wa = ta + parts.start(warp), wb = ta + parts.start(warp + 1), n = wb - wa;
 
-    // ---- this warp's tiles ----
-    if (n > 0) {
-        const uint8_t *src = nullptr;  // lane i: tile base + i
-        auto look_up = [&](int base) {
-            const int t = wa + base + lane;
-            if (t >= wb) return;
-            const int s = take_of(pre, B, t), T = tiles_of(Ls[s]), off = t - pre[s], kh = off / T, j = off - kh * T;
-            int page = P.table[static_cast<long>(s) * P.maxpages + j / 2];
-            if (page < 0 || page >= P.npages) {
-                record_error(OUMU_DEVERR_PAGE);
-                page = 0;  // read in its place: the take's output is unspecified
-            }
-            src = P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + (j & 1) * F::HALFB;
-        };
-        auto issue = [&](int k) {  // tile k into its stage
-            const unsigned long long a = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k & 31);
-            if (lane == 0) {
-                const uint32_t bar = bars + 8 * (k % ST);
-                mbar_expect_tx(bar, F::HALFB);
-                bulk_load(ring + (k % ST) * F::HALFB, reinterpret_cast<const void *>(a), F::HALFB, bar);
-            }
-        };
-        look_up(0);
-        issue(0);
-        int s = take_of(pre, B, wa), T = tiles_of(Ls[s]), kh = (wa - pre[s]) / T, j = wa - pre[s] - kh * T;
-        Query<HD> Q;
-        State<HD> S;
-        Newest<HD> N;
-        bool ok = true, fresh = true;
-        int issued = n < ST ? n : ST;
-        for (int k = 0; k < n; k++) {
-            const int L = Ls[s];
-            if (fresh) {
-                Q.load(P, s, kh, L - 1, lane);
-                S.clear();
-                if (FUSED && T - 1 - j < n - k) {  // the segment's last tile is this warp's
-                    const int page = P.table[static_cast<long>(s) * P.maxpages + (T - 1) / 2];
-                    if (page >= 0 && page < P.npages)
-                        N.make(P, s, kh, L - 1, lane,
-                               P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + ((T - 1) & 1) * F::HALFB);
-                }
-                fresh = false;
-            }
-            if (k == 0)  // the first tile went ahead; the others follow behind every warp's first
-                for (int i = 1; i < ST && i < n; i++) issue(i);
-            const uint32_t bar = bars + 8 * (k % ST), phase = (k / ST) & 1;
-            if (!__all_sync(0xffffffffu, ok && mbar_try_wait(bar, phase)))
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, phase));
-            if (ok) {
-                uint8_t *half = sm + warp * Y::RING + (k % ST) * F::HALFB;
-                if (FUSED && j == T - 1) {
-                    N.patch(half, (L - 1) % HALF, lane);
-                    fence_proxy_async_smem();  // before the stage's next copy
-                    __syncwarp();
-                }
-                S.tile(half, L - j * HALF, Q, lane);
-            }
-            __syncwarp();
-            if (k + ST < n) {
-                if (((k + ST) & 31) == 0) look_up(k + ST);
-                if (ok) {
-                    issue(k + ST);
-                    issued++;
-                }
-            }
-            if (j == T - 1 || k == n - 1) {
-                // ---- the segment's end, or this warp's ----
-                const int Sg = wa + k - j;
-                if (Sg >= wa && j == T - 1) {
-                    S.finish(P.out + (static_cast<long>(s) * P.nq + kh * G) * HD, G, lane);
-                } else {
-                    float *R = k == n - 1 ? reinterpret_cast<float *>(sm + warp * Y::RING)
-                                          : reinterpret_cast<float *>(sm + Y::FIRST) + warp * Y::REC;
-                    S.record(R, lane);
-                }
-                fresh = true;
-            }
-            if (++j == T) {
-                j = 0;
-                if (++kh == nk) {
-                    kh = 0;
-                    do ++s; while (s < B && Ls[s] == 0);
-                    T = s < B ? tiles_of(Ls[s]) : 1;
-                }
-            }
-        }
-        if (!ok)  // after a wait that ran out: no copy may still be on its way when the CTA leaves (bounded again)
-            for (int k = issued > ST ? issued - ST : 0; k < issued; k++) mbar_wait(bars + 8 * (k % ST), (k / ST) & 1);
-    }
-    __syncthreads();
-
-    // ---- segments that cross a boundary between warps, or the CTA's ends ----
-    // Warp 0 lists them: boundary b (where warp b starts; b == NW: the CTA's end) lies inside one, unless it is the one
-    // before it again. The loops below are not unrolled: run once per launch, they cost their instruction fetches.
     Cross *list = reinterpret_cast<Cross *>(sm + Y::LIST);
-    if (warp == 0) {
+    auto list_crossings = [&] {
+        // Boundary b (where warp b starts; b == NW: the CTA's end) lies inside a segment, which may be the one before it
+        // again, or between two.
         Cross x{-1, 0, 0, 0, 0};
         const int at = ta + parts.start(lane < NW ? lane : NW);
         const bool any = lane < NW ? at < tb : lane == NW;  // a warp without tiles starts where the CTA ends
@@ -769,8 +682,90 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
             list[__popc(in & ((1u << lane) - 1))] = x;
         }
         if (lane == 0) misc[0] = __popc(in);
+    };
+    // ---- this warp's tiles ----
+    if (n > 0) {
+        const uint8_t *src = nullptr;  // lane i: tile base + i
+        auto look_up = [&](int base) {
+            const int t = wa + base + lane;
+            if (t >= wb) return;
+            const int s = take_of(pre, B, t), T = tiles_of(Ls[s]), off = t - pre[s], kh = off / T, j = off - kh * T;
+            int page = P.table[static_cast<long>(s) * P.maxpages + j / 2];
+            if (page < 0 || page >= P.npages) {
+                record_error(OUMU_DEVERR_PAGE);
+                page = 0;  // read in its place: the take's output is unspecified
+            }
+            src = P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + (j & 1) * F::HALFB;
+        };
+        auto issue = [&](int k) {  // tile k into its stage
+            const unsigned long long a = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k & 31);
+            bulk_load_first_lane(ring + (k % ST) * F::HALFB, a, F::HALFB, bars + 8 * (k % ST), lane);
+        };
+        look_up(0);
+        issue(0);
+        if (warp == 0) list_crossings();  // while the first copies are on their way
+        int s = take_of(pre, B, wa), T = tiles_of(Ls[s]), kh = (wa - pre[s]) / T, j = wa - pre[s] - kh * T;
+        int k = 0, issued = 1;
+        while (k < n) {
+            // ---- this warp's part of a segment: tiles j .. of take s, kv head kh ----
+            const int L = Ls[s], Sg = wa + k - j, stop = min(n, k + T - j);
+            Query<HD> Q;
+            State<HD> S;
+            Newest<HD> N;
+            Q.load(P, s, kh, L - 1, lane);
+            S.clear();
+            const bool ends = stop == k + T - j;  // its last tile is this warp's
+            if (FUSED && ends) {
+                const int page = P.table[static_cast<long>(s) * P.maxpages + (T - 1) / 2];
+                if (page >= 0 && page < P.npages)
+                    N.make(P, s, kh, L - 1, lane,
+                           P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + ((T - 1) & 1) * F::HALFB);
+            }
+            for (; issued < ST && issued < n; issued++) issue(issued);  // behind every warp's first tile
+            int left = L - j * HALF;  // positions from this tile on
+            for (; k < stop; k++, left -= HALF) {
+                const uint32_t bar = bars + 8 * (k % ST), phase = (k / ST) & 1;
+                if (!__all_sync(0xffffffffu, mbar_try_wait(bar, phase)) &&
+                    !__all_sync(0xffffffffu, mbar_wait(bar, phase)))
+                    break;
+                uint8_t *half = sm + warp * Y::RING + (k % ST) * F::HALFB;
+                if (FUSED && ends && k == stop - 1) {
+                    N.patch(half, (L - 1) % HALF, lane);
+                    fence_proxy_async_smem();  // before the stage's next copy
+                    __syncwarp();
+                }
+                S.tile(half, left, Q, lane);
+                __syncwarp();
+                if (issued < n) {
+                    if ((issued & 31) == 0) look_up(issued);
+                    issue(issued++);
+                }
+            }
+            if (k < stop) {
+                // A wait ran out (recorded): nothing more is computed or started; the outputs are unspecified, but no
+                // copy may still be on its way when the CTA leaves (bounded again).
+                for (int i = k; i < issued; i++) mbar_wait(bars + 8 * (i % ST), (i / ST) & 1);
+                break;
+            }
+            if (ends && Sg >= wa) {
+                S.finish(P.out + (static_cast<long>(s) * P.nq + kh * G) * HD, G, lane);
+            } else {
+                S.record(k == n ? reinterpret_cast<float *>(sm + warp * Y::RING)
+                                : reinterpret_cast<float *>(sm + Y::FIRST) + warp * Y::REC,
+                         lane);
+            }
+            j = 0;
+            if (++kh == nk) {
+                kh = 0;
+                do ++s; while (s < B && Ls[s] == 0);
+                T = s < B ? tiles_of(Ls[s]) : 1;
+            }
+        }
     }
     __syncthreads();
+
+    // ---- segments that cross a boundary between warps, or the CTA's ends ----
+    // The loops here are not unrolled: run once per launch, they cost their instruction fetches.
     const int nlist = misc[0];
     constexpr int LPH = HD / 4;  // threads per head, 4 channels each
     const int h = threadIdx.x / LPH, d4 = threadIdx.x % LPH;
@@ -796,15 +791,25 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
             return x.end >= ta + parts.start(w + 1) ? reinterpret_cast<const float *>(sm + w * Y::RING)
                                                     : reinterpret_cast<const float *>(sm + Y::FIRST) + w * Y::REC;
         };
-        float M = -INFINITY, l = 0.f;
+        // the head's LPH threads take a record's reference and sum each
+        const unsigned mates = LPH == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
+        const bool has = x.first + d4 <= x.last;
+        const float m = has ? at(x.first + d4)[h] : -INFINITY;
+        float M = m;
+#pragma unroll
+        for (int e = 1; e < 16; e <<= 1) M = fmaxf(M, __shfl_xor_sync(mates, M, e, 16));
+        M = __shfl_sync(mates, M, 0, LPH);
+        const float fm = fast_exp2(m - M);
+        float l = has ? fm * at(x.first + d4)[GMAX + h] : 0.f;
+#pragma unroll
+        for (int e = 1; e < 16; e <<= 1) l += __shfl_xor_sync(mates, l, e, 16);
+        l = __shfl_sync(mates, l, 0, LPH);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-        for (int w = x.first; w <= x.last; w++) M = fmaxf(M, at(w)[h]);
-#pragma unroll 1
+#pragma unroll 2
         for (int w = x.first; w <= x.last; w++) {
-            const float *R = at(w);
-            add(fast_exp2(R[h] - M), R[GMAX + h], *reinterpret_cast<const float4 *>(R + 2 * GMAX + h * HD + 4 * d4), l,
-                o);
+            const float f = __shfl_sync(mates, fm, w - x.first, LPH);
+            const float4 v = *reinterpret_cast<const float4 *>(at(w) + 2 * GMAX + h * HD + 4 * d4);
+            o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
         }
         if (!out) {
             store(x.id, l, o);
