@@ -500,11 +500,9 @@ struct Newest {
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) rg = kv4::range_max(rg, __shfl_xor_sync(0xffffffffu, rg, o));
             const kv4::Quant q = kv4::quant_of(rg);
-            const float2 a = unpack_bf16x2(u[kv].x), b = unpack_bf16x2(u[kv].y);
-            const uint32_t n[4] = {static_cast<uint32_t>(kv4::quant_code(a.x, q)),
-                                   static_cast<uint32_t>(kv4::quant_code(a.y, q)),
-                                   static_cast<uint32_t>(kv4::quant_code(b.x, q)),
-                                   static_cast<uint32_t>(kv4::quant_code(b.y, q))};
+            const uint32_t pr[2] = {u[kv].x, u[kv].y};
+            const uint32_t c = kv4::quant_pairs<2>(pr, q);  // low half: channels 0, 2; high half: 1, 3
+            const uint32_t n[4] = {c & 15u, c >> 16 & 15u, c >> 4 & 15u, c >> 20 & 15u};
             if (P.held && on) {
                 uint2 o;
                 o.x = pack_bf16x2(fmaf(q.s, n[0], q.z), fmaf(q.s, n[1], q.z));
@@ -512,7 +510,7 @@ struct Newest {
                 *reinterpret_cast<uint2 *>(P.held + (static_cast<long>(s) * 2 * P.nk + kv * P.nk + kh) * HD + c4) = o;
             }
             if (kv == 0) {  // two bytes of the word that lanes j and j ^ 1 share
-                const uint32_t kw = (n[0] | n[2] << 4 | (n[1] | n[3] << 4) << 16) << (8 * (j & 1));
+                const uint32_t kw = (c & 0x00ff00ffu) << (8 * (j & 1));
                 code[0] = kw | __shfl_xor_sync(0xffffffffu, kw, 1);
             } else {
                 code[1] = n[0] | n[1] << 4 | n[2] << 8 | n[3] << 12;

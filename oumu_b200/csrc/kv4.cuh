@@ -83,36 +83,78 @@ __device__ __forceinline__ uint32_t range_max(uint32_t a, uint32_t b) { return a
 struct Quant {
     float s, z, rinv;
 };
-// Rounding up twice in fp32 (x - y, then / 15) and then to bf16 gives the smallest bf16 >= (max - min) / 15 itself:
-// if a bf16 b is >= it, 15 b is >= max - min and has 12 bits, so neither step rounds past it.
+// s, the smallest bf16 >= D / 15 with D = max - min rounded up in fp32 (15 s has 12 bits, so rounding D up to fp32 does
+// not change which s is enough): D times a float a little above 1 / 15, cut to bf16, is it or the one before it, and
+// 15 s >= D, exact, tells. A scale that is not finite becomes NaN.
 __device__ __forceinline__ Quant quant_of(uint32_t range) {
     const float2 r = unpack_bf16x2(range);  // max, -min
     Quant q;
     q.z = -r.y;
-    const float d = __fdiv_ru(__fadd_ru(r.x, r.y), 15.f);
-    q.s = d != d ? d : __uint_as_float((__float_as_uint(d) + 0xffffu) & 0xffff0000u);
+    const float D = __fadd_ru(r.x, r.y);
+    const uint32_t b = __float_as_uint(D * __uint_as_float(0x3d88888au)) & 0xffff0000u;
+    q.s = __uint_as_float(15.f * __uint_as_float(b) >= D ? b : b + 0x10000u);
+    if (!(D < 3.4e38f)) q.s = __uint_as_float(0x7fc00000u);
     q.rinv = __fdividef(1.f, q.s);
     return q;
 }
-// Nearest multiple near a border: x - z = d + e exactly (two-sum), r = d - n s exactly (n s has 12 bits).
-__device__ __noinline__ int quant_exact(float x, float z, float s) {
-    if (!(s > 0.f) || !(s < INFINITY)) return 0;
-    const float d = __fsub_rn(x, z);
+// The nearest multiple decided exactly, for a group of which some value lies on a border (among bf16 numbers ties are
+// common) or whose scale has no normal reciprocal: x - z = d + e (two-sum), r = d - n s exactly (n s has 12 bits, n is
+// at most one off).
+__device__ __forceinline__ uint32_t quant_exact(float x, const Quant &q) {
+    const float d = __fsub_rn(x, q.z);
     const float bb = __fsub_rn(d, x);
-    const float e = __fadd_rn(__fsub_rn(x, __fsub_rn(d, bb)), __fsub_rn(-z, bb));
-    float n = rintf(__fdiv_rn(d, s));
-    const float r = fmaf(-n, s, d), h = 0.5f * s;
+    const float e = __fadd_rn(__fsub_rn(x, __fsub_rn(d, bb)), __fsub_rn(-q.z, bb));
+    float n = fminf(fmaxf(rintf(q.rinv < 1.7e38f ? d * q.rinv : __fdiv_rn(d, q.s)), 0.f), 15.f);
+    const float r = fmaf(-n, q.s, d), h = 0.5f * q.s;
     const bool odd = static_cast<int>(n) & 1;
     if (r > h || (r == h && (e > 0.f || (e == 0.f && odd)))) n += 1.f;
     else if (r < -h || (r == -h && (e < 0.f || (e == 0.f && odd)))) n -= 1.f;
-    return static_cast<int>(fminf(fmaxf(n, 0.f), 15.f));
+    return q.s > 0.f ? static_cast<uint32_t>(n) : 0u;
 }
-// The product with 1 / s is within 2^-21 of the quotient (at most 15): away from a border by more, rounding it is right.
-__device__ __forceinline__ int quant_code(float x, const Quant &q) {
-    const float t = __fsub_rn(x, q.z) * q.rinv;
-    const float n = rintf(t);
-    if (fabsf(t - n) < 0.4999f) return static_cast<int>(n);
-    return quant_exact(x, q.z, q.s);  // NaN and infinities of the product come here too
+template <int NP>
+__device__ __noinline__ uint32_t quant_pairs_exact(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, Quant q) {
+    const uint32_t x[4] = {x0, x1, x2, x3};
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int i = NP - 1; i >= 0; i--) {
+        const float2 f = unpack_bf16x2(x[i]);
+        lo = lo * 16u + quant_exact(f.x, q);
+        hi = hi * 16u + quant_exact(f.y, q);
+    }
+    return lo | hi << 16;
+}
+// The codes of NP bf16 pairs, nibble i of the low and high half being pair i's two values. The quotient (x - z) / s is
+// corrected to the nearest float, so a tie among whole numbers is one exactly and adding 1.5 * 2^23 rounds it to even (n
+// is then in the low bits). Each n is right where the remainder is below s / 2, or s / 2 itself and x - z exact.
+template <int NP>
+__device__ __forceinline__ uint32_t quant_pairs(const uint32_t (&x)[NP], const Quant &q) {
+    const float magic = 12582912.f, h = 0.5f * q.s;
+    const float2 rv = make_float2(q.rinv, q.rinv), ms = make_float2(-q.s, -q.s);
+    const float2 mz = make_float2(-q.z, -q.z), mg = make_float2(magic, magic), back = make_float2(-magic, -magic);
+    uint32_t lo = 0, hi = 0;
+    float far = 0.f;
+    float2 f[NP], d[NP], r[NP];
+#pragma unroll
+    for (int i = NP - 1; i >= 0; i--) {
+        f[i] = make_float2(__uint_as_float(x[i] << 16), __uint_as_float(x[i] & 0xffff0000u));
+        d[i] = add2(f[i], mz);
+        const float2 t = mul2(d[i], rv);
+        const float2 a = add2(fma2(fma2(t, ms, d[i]), rv, t), mg);
+        r[i] = fma2(add2(a, back), ms, d[i]);
+        far = fmax3(far, fabsf(r[i].x), fabsf(r[i].y));
+        lo = lo * 16u + __float_as_uint(a.x);  // the magic number's own bits leave the low 16
+        hi = hi * 16u + __float_as_uint(a.y);
+    }
+    const bool normal = q.rinv < 1.7e38f;  // not for scales of 0 or below 2^-127
+    if (!(far < h && normal)) {
+        // a tie (among bf16 numbers common), or something rarer
+        bool odd = !(far <= h && normal);
+#pragma unroll
+        for (int i = 0; i < NP; i++)
+            odd = odd || __fadd_rn(d[i].x, q.z) != f[i].x || __fadd_rn(d[i].y, q.z) != f[i].y;
+        if (odd) return quant_pairs_exact<NP>(x[0], x[1], x[NP - 2], x[NP - 1], q);
+    }
+    return __byte_perm(lo, hi, 0x5410);
 }
 __device__ __forceinline__ uint32_t meta_bits(float a, float b) {  // two bf16-valued floats as a bf16 pair
     return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
@@ -132,124 +174,153 @@ __device__ __forceinline__ uint8_t *unit_of(uint8_t *pool, const int *table, int
 
 // ---- prompt writes and reads -----------------------------------------------------------------------------------
 
-// One warp per (take, block of 8 positions, kv head, K or V). Bound by HBM (512 bytes read and 160 written per
-// position and kv head at hd 128); the lanes load q-row chunks in the order of the block's words, so the block's
-// 512 bytes of codes leave in one 16-byte store per lane.
+// Work of one warp: `per` blocks of 8 positions of one (take, kv head, K or V), aligned inside a page; the next block's
+// rows are on their way while one is worked on.
+struct Part {
+    int s, h, v, block;  // v: 0 for K, 1 for V; the first block
+    __device__ Part(long item, int parts, int nk) {
+        const int hv = static_cast<int>(item % (2 * nk));
+        const long sp = item / (2 * nk);
+        h = hv >> 1;
+        v = hv & 1;
+        s = static_cast<int>(sp / parts);
+        block = static_cast<int>(sp % parts);
+    }
+};
+
+// Bound by HBM: 512 bytes read and 160 written per position and kv head at hd 128. The lanes load row chunks in the order
+// of the block's words, so a block's 512 bytes of codes leave in one 16-byte store per lane.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv4_write(const bf16 *qkv, uint8_t *pool, const int *table, const int *start,
                                                    const int *count, int B, int rows, int nq, int nk, int npages,
-                                                   int maxpages, int blocks) {
+                                                   int maxpages, int parts, int per) {
     using F = Fmt<HD>;
     constexpr int W = F::W;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const long item = static_cast<long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const int hv = static_cast<int>(item % (2 * nk)), h = hv >> 1;
-    const long sb = item / (2 * nk);
-    const int s = static_cast<int>(sb / blocks), b = static_cast<int>(sb % blocks);
-    if (s >= B) return;
-    const int p0 = start ? start[s] : 0, n = count ? min(count[s], rows) : rows;
+    const Part it(static_cast<long>(blockIdx.x) * 8 + (threadIdx.x >> 5), parts, nk);
+    if (it.s >= B) return;
+    const int p0 = start ? start[it.s] : 0, n = count ? min(count[it.s], rows) : rows;
     if (n <= 0) return;
     if (p0 < 0 || static_cast<long>(p0) + n > static_cast<long>(maxpages) * PAGE) {
-        if (lane == 0 && b == 0) record_error(OUMU_DEVERR_LENGTH);
+        if (lane == 0 && it.block == 0) record_error(OUMU_DEVERR_LENGTH);
         return;
     }
-    const int pb = (p0 / 8 + b) * 8;  // the block's first position
-    if (pb >= p0 + n) return;
-    uint8_t *u = unit_of(pool, table, s, pb, h, nk, npages, maxpages, F::UNIT);
+    const int b0 = (p0 / (8 * per) + it.block) * per;
+    const int first = max(b0, p0 / 8), last = min(b0 + per - 1, (p0 + n - 1) / 8);  // blocks with rows to write
+    if (first > last) return;
+    uint8_t *u = unit_of(pool, table, it.s, b0 * 8, it.h, nk, npages, maxpages, F::UNIT);
     if (!u) return;
-    u += (pb % PAGE) / HALF * F::HALFB;
-    const int r0 = pb % HALF;
     const long pitch = static_cast<long>(nq + 2 * nk) * HD;
-    const bf16 *src = qkv + (static_cast<long>(s) * rows + pb - p0) * pitch + (nq + (hv & 1) * nk + h) * HD;
-    auto ok = [&](int i) { return pb + i >= p0 && pb + i < p0 + n; };
-    Words<W> code, meta;
-    if (!(hv & 1)) {  // K: lane 4g + t has channels 32w + 8t .. + 7 of position g
-        uint4 x[W];
-#pragma unroll
-        for (int w = 0; w < W; w++)
-            x[w] = ok(g) ? *reinterpret_cast<const uint4 *>(src + g * pitch + 32 * w + 8 * t) : make_uint4(0, 0, 0, 0);
-        uint32_t sc[W], zc[W];
-#pragma unroll
-        for (int w = 0; w < W; w++) {
-            const uint32_t *xu = reinterpret_cast<const uint32_t *>(&x[w]);
-            uint32_t mx = xu[0], mn = xu[0];
-#pragma unroll
-            for (int i = 1; i < 4; i++) {
-                mx = as_u32(__hmax2_nan(as_bf2(mx), as_bf2(xu[i])));
-                mn = as_u32(__hmin2_nan(as_bf2(mn), as_bf2(xu[i])));
-            }
-            uint32_t rg = range_of(mx, mn);
-            rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, 1));
-            rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, 2));
-            const Quant q = quant_of(rg);
-            uint32_t c = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 f = unpack_bf16x2(xu[i]);
-                c |= static_cast<uint32_t>(quant_code(f.x, q)) << (4 * i);
-                c |= static_cast<uint32_t>(quant_code(f.y, q)) << (4 * i + 16);
-            }
-            code.v[w] = c;
-            sc[w] = __float_as_uint(q.s) >> 16;
-            zc[w] = __float_as_uint(q.z) >> 16;
-        }
-        if (!ok(g)) return;
-        st_words<W>(u + r0 / 8 * F::BLOCK + lane * 4 * W, code);
-#pragma unroll
-        for (int w = 0; w < W; w += 2) {
-            meta.v[w / 2] = sc[w] | sc[w + 1] << 16;
-            meta.v[W / 2 + w / 2] = zc[w] | zc[w + 1] << 16;
-        }
-        if (t == 0) st_words<W>(u + F::KMETA + (r0 + g) * F::ROW, meta);
-    } else {  // V: lane 4g + t has channels 32w + 4g .. + 3 of positions 2t and 2t + 1
-        uint2 x[2][W];
-#pragma unroll
-        for (int e = 0; e < 2; e++)
+    const bf16 *src = qkv + (static_cast<long>(it.s) * rows - p0) * pitch + (nq + it.v * nk + it.h) * HD;
+    auto ok = [&](int p) { return p >= p0 && p < p0 + n; };
+    if (it.v == 0) {  // K: lane 4g + t has channels 32w + 8t .. + 7 of position g
+        auto load = [&](int b, uint4 (&x)[W]) {
+            const int p = b * 8 + g;
 #pragma unroll
             for (int w = 0; w < W; w++)
-                x[e][w] = ok(2 * t + e) ? *reinterpret_cast<const uint2 *>(src + (2 * t + e) * pitch + 32 * w + 4 * g)
-                                        : make_uint2(0, 0);
-        uint32_t sc[2][W], zc[2][W];
+                x[w] = ok(p) ? __ldcs(reinterpret_cast<const uint4 *>(src + p * pitch + 32 * w + 8 * t))
+                             : make_uint4(0, 0, 0, 0);
+        };
+        uint4 y[W];
+        load(first, y);
+        for (int b = first; b <= last; b++) {
+            uint4 x[W];
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            code.v[w] = 0;
+            for (int w = 0; w < W; w++) x[w] = y[w];
+            if (b < last) load(b + 1, y);
+            Words<W> code, meta;
+            uint32_t sz[W];
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const uint2 y = x[e][w];
-                uint32_t rg = range_of(as_u32(__hmax2_nan(as_bf2(y.x), as_bf2(y.y))),
-                                       as_u32(__hmin2_nan(as_bf2(y.x), as_bf2(y.y))));
+            for (int w = 0; w < W; w++) {
+                const uint32_t xu[4] = {x[w].x, x[w].y, x[w].z, x[w].w};
+                uint32_t mx = xu[0], mn = xu[0];
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, o));
+                for (int i = 1; i < 4; i++) {
+                    mx = as_u32(__hmax2_nan(as_bf2(mx), as_bf2(xu[i])));
+                    mn = as_u32(__hmin2_nan(as_bf2(mn), as_bf2(xu[i])));
+                }
+                uint32_t rg = range_of(mx, mn);
+                rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, 1));
+                rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, 2));
                 const Quant q = quant_of(rg);
-                const float2 a = unpack_bf16x2(y.x), c = unpack_bf16x2(y.y);
-                const uint32_t n4 = quant_code(a.x, q) | quant_code(a.y, q) << 4 | quant_code(c.x, q) << 8 |
-                                    quant_code(c.y, q) << 12;
-                code.v[w] |= n4 << (16 * e);
-                sc[e][w] = __float_as_uint(q.s) >> 16;
-                zc[e][w] = __float_as_uint(q.z) >> 16;
+                code.v[w] = quant_pairs<4>(xu, q);
+                sz[w] = meta_bits(q.s, q.z);
             }
-        }
-        uint8_t *dst = u + F::CODES + r0 / 8 * F::BLOCK + lane * 4 * W;
-        if (ok(2 * t) && ok(2 * t + 1)) {
-            st_words<W>(dst, code);
-        } else {  // one of the word's two positions belongs to this write: its halves only
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-                if (ok(2 * t + e))
-#pragma unroll
-                    for (int w = 0; w < W; w++)
-                        reinterpret_cast<uint16_t *>(dst)[2 * w + e] = static_cast<uint16_t>(code.v[w] >> (16 * e));
-        }
-        if (g == 0) {
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                if (!ok(2 * t + e)) continue;
+            if (!ok(b * 8 + g)) continue;
+            uint8_t *half = u + (b & 7) / 4 * F::HALFB;
+            st_words<W>(half + (b & 3) * F::BLOCK + lane * 4 * W, code);
+            if (t == 0) {
 #pragma unroll
                 for (int w = 0; w < W; w += 2) {
-                    meta.v[w / 2] = sc[e][w] | sc[e][w + 1] << 16;
-                    meta.v[W / 2 + w / 2] = zc[e][w] | zc[e][w + 1] << 16;
+                    meta.v[w / 2] = __byte_perm(sz[w], sz[w + 1], 0x5410);
+                    meta.v[W / 2 + w / 2] = __byte_perm(sz[w], sz[w + 1], 0x7632);
                 }
-                st_words<W>(u + F::VMETA + (r0 + 2 * t + e) * F::ROW, meta);
+                st_words<W>(half + F::KMETA + ((b & 3) * 8 + g) * F::ROW, meta);
+            }
+        }
+    } else {  // V: lane 4g + t has channels 32w + 4g .. + 3 of positions 2t and 2t + 1
+        auto load = [&](int b, uint2 (&x)[2][W]) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int p = b * 8 + 2 * t + e;
+#pragma unroll
+                for (int w = 0; w < W; w++)
+                    x[e][w] = ok(p) ? __ldcs(reinterpret_cast<const uint2 *>(src + p * pitch + 32 * w + 4 * g))
+                                    : make_uint2(0, 0);
+            }
+        };
+        uint2 y[2][W];
+        load(first, y);
+        for (int b = first; b <= last; b++) {
+            uint2 x[2][W];
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int w = 0; w < W; w++) x[e][w] = y[e][w];
+            if (b < last) load(b + 1, y);
+            Words<W> code, meta;
+            uint32_t sz[2][W];
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                uint32_t n4[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint2 v = x[e][w];
+                    uint32_t rg = range_of(as_u32(__hmax2_nan(as_bf2(v.x), as_bf2(v.y))),
+                                           as_u32(__hmin2_nan(as_bf2(v.x), as_bf2(v.y))));
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, o));
+                    const Quant q = quant_of(rg);
+                    const uint32_t pr[2] = {v.x, v.y};
+                    const uint32_t c = quant_pairs<2>(pr, q);  // low half: channels 0, 2; high half: 1, 3
+                    n4[e] = (c & 0xfu) | (c >> 12 & 0xf0u) | (c << 4 & 0xf00u) | (c >> 8 & 0xf000u);
+                    sz[e][w] = meta_bits(q.s, q.z);
+                }
+                code.v[w] = __byte_perm(n4[0], n4[1], 0x5410);
+            }
+            uint8_t *half = u + (b & 7) / 4 * F::HALFB;
+            uint8_t *dst = half + F::CODES + (b & 3) * F::BLOCK + lane * 4 * W;
+            const bool ok0 = ok(b * 8 + 2 * t), ok1 = ok(b * 8 + 2 * t + 1);
+            if (ok0 && ok1) {
+                st_words<W>(dst, code);
+            } else {  // one of the word's two positions belongs to this write: its halves only
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    if (ok0) reinterpret_cast<uint16_t *>(dst)[2 * w] = static_cast<uint16_t>(code.v[w]);
+                    if (ok1) reinterpret_cast<uint16_t *>(dst)[2 * w + 1] = static_cast<uint16_t>(code.v[w] >> 16);
+                }
+            }
+            if (g == 0) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    if (!(e ? ok1 : ok0)) continue;
+#pragma unroll
+                    for (int w = 0; w < W; w += 2) {
+                        meta.v[w / 2] = __byte_perm(sz[e][w], sz[e][w + 1], 0x5410);
+                        meta.v[W / 2 + w / 2] = __byte_perm(sz[e][w], sz[e][w + 1], 0x7632);
+                    }
+                    st_words<W>(half + F::VMETA + ((b & 3) * 8 + 2 * t + e) * F::ROW, meta);
+                }
             }
         }
     }
@@ -258,63 +329,71 @@ __global__ void __launch_bounds__(256) k_kv4_write(const bf16 *qkv, uint8_t *poo
 // The 4 codes of nibbles 0..3 of a 16-bit half, as values rounded once to bf16 (s n is exact, the sum rounds once
 // in fp32 and once to bf16).
 __device__ __forceinline__ float value_of(uint32_t half, int i, float s, float z) {
-    return fmaf(s, static_cast<float>((half >> (4 * i)) & 15u), z);
+    // n from its bits: 2^23 + n, minus 2^23
+    return fmaf(s, __uint_as_float(((half >> (4 * i)) & 15u) | 0x4b000000u) - 8388608.f, z);
 }
 
-// One warp per (take, block of 8 positions, kv head, K or V), the write's order backwards.
-template <int HD>
+// The write's order backwards; a part's codes and meta rows are all loaded before the first value is stored.
+template <int HD, int PER>
 __global__ void __launch_bounds__(256) k_kv4_read(uint8_t *pool, const int *table, const int *lens, const int *pos,
                                                   bf16 *kc, bf16 *vc, int B, int nk, int npages, int maxpages,
-                                                  int maxlen, int blocks) {
+                                                  int maxlen, int parts) {
     using F = Fmt<HD>;
     constexpr int W = F::W;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const long item = static_cast<long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const int hv = static_cast<int>(item % (2 * nk)), h = hv >> 1;
-    const long sb = item / (2 * nk);
-    const int s = static_cast<int>(sb / blocks), b = static_cast<int>(sb % blocks);
-    if (s >= B) return;
-    int L = lens ? lens[s] : *pos + 1;
+    const Part it(static_cast<long>(blockIdx.x) * 8 + (threadIdx.x >> 5), parts, nk);
+    if (it.s >= B) return;
+    int L = lens ? lens[it.s] : *pos + 1;
     const long room = min(static_cast<long>(maxlen), static_cast<long>(maxpages) * PAGE);
     if (L < 0 || L > room) {
-        if (lane == 0 && b == 0) record_error(OUMU_DEVERR_LENGTH);
+        if (lane == 0 && it.block == 0) record_error(OUMU_DEVERR_LENGTH);
         L = L < 0 ? 0 : static_cast<int>(room);
     }
-    const int pb = b * 8;
-    if (pb >= L) return;
-    const uint8_t *u = unit_of(pool, table, s, pb, h, nk, npages, maxpages, F::UNIT);
+    const int b0 = it.block * PER;
+    if (b0 * 8 >= L) return;
+    const uint8_t *u = unit_of(pool, table, it.s, b0 * 8, it.h, nk, npages, maxpages, F::UNIT);
     if (!u) return;
-    u += (pb % PAGE) / HALF * F::HALFB;
-    const int r0 = pb % HALF;
-    const Words<W> code = ld_words<W>(u + (hv & 1) * F::CODES + r0 / 8 * F::BLOCK + lane * 4 * W);
-    bf16 *dst = (hv & 1 ? vc : kc) + ((static_cast<long>(s) * nk + h) * maxlen + pb) * HD;
-    if (!(hv & 1)) {
-        if (pb + g >= L) return;
-        const Words<W> m = ld_words<W>(u + F::KMETA + (r0 + g) * F::ROW);
+    u += (b0 & 7) / 4 * F::HALFB;
+    bf16 *dst = (it.v ? vc : kc) + ((static_cast<long>(it.s) * nk + it.h) * maxlen + b0 * 8) * HD;
+    const int left = L - b0 * 8;
+    Words<W> code[PER], m[PER][2];
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            const float sc = row_scale<W>(m, w), z = row_zero<W>(m, w);
-            const uint32_t lo = code.v[w] & 0xffffu, hi = code.v[w] >> 16;
-            uint4 o;
-            o.x = pack_bf16x2(value_of(lo, 0, sc, z), value_of(hi, 0, sc, z));
-            o.y = pack_bf16x2(value_of(lo, 1, sc, z), value_of(hi, 1, sc, z));
-            o.z = pack_bf16x2(value_of(lo, 2, sc, z), value_of(hi, 2, sc, z));
-            o.w = pack_bf16x2(value_of(lo, 3, sc, z), value_of(hi, 3, sc, z));
-            *reinterpret_cast<uint4 *>(dst + g * HD + 32 * w + 8 * t) = o;
-        }
-    } else {
+    for (int i = 0; i < PER; i++) {
+        if (i * 8 >= left) break;
+        code[i] = ld_words<W>(u + it.v * F::CODES + ((b0 + i) & 3) * F::BLOCK + lane * 4 * W);
+        const uint8_t *rows = u + (it.v ? F::VMETA : F::KMETA) + ((b0 + i) & 3) * 8 * F::ROW;
+        m[i][0] = ld_words<W>(rows + (it.v ? 2 * t : g) * F::ROW);
+        if (it.v) m[i][1] = ld_words<W>(rows + (2 * t + 1) * F::ROW);
+    }
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            if (pb + 2 * t + e >= L) continue;
-            const Words<W> m = ld_words<W>(u + F::VMETA + (r0 + 2 * t + e) * F::ROW);
+    for (int i = 0; i < PER; i++) {
+        if (i * 8 >= left) break;
+        if (it.v == 0) {
+            if (i * 8 + g >= left) continue;
 #pragma unroll
             for (int w = 0; w < W; w++) {
-                const float sc = row_scale<W>(m, w), z = row_zero<W>(m, w);
-                const uint32_t hf = code.v[w] >> (16 * e) & 0xffffu;
-                uint2 o;
-                o.x = pack_bf16x2(value_of(hf, 0, sc, z), value_of(hf, 1, sc, z));
-                o.y = pack_bf16x2(value_of(hf, 2, sc, z), value_of(hf, 3, sc, z));
-                *reinterpret_cast<uint2 *>(dst + (2 * t + e) * HD + 32 * w + 4 * g) = o;
+                const float sc = row_scale<W>(m[i][0], w), z = row_zero<W>(m[i][0], w);
+                const uint32_t lo = code[i].v[w] & 0xffffu, hi = code[i].v[w] >> 16;
+                uint4 o;
+                o.x = pack_bf16x2(value_of(lo, 0, sc, z), value_of(hi, 0, sc, z));
+                o.y = pack_bf16x2(value_of(lo, 1, sc, z), value_of(hi, 1, sc, z));
+                o.z = pack_bf16x2(value_of(lo, 2, sc, z), value_of(hi, 2, sc, z));
+                o.w = pack_bf16x2(value_of(lo, 3, sc, z), value_of(hi, 3, sc, z));
+                __stcs(reinterpret_cast<uint4 *>(dst + (i * 8 + g) * HD + 32 * w + 8 * t), o);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                if (i * 8 + 2 * t + e >= left) continue;
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    const float sc = row_scale<W>(m[i][e], w), z = row_zero<W>(m[i][e], w);
+                    const uint32_t hf = code[i].v[w] >> (16 * e) & 0xffffu;
+                    uint2 o;
+                    o.x = pack_bf16x2(value_of(hf, 0, sc, z), value_of(hf, 1, sc, z));
+                    o.y = pack_bf16x2(value_of(hf, 2, sc, z), value_of(hf, 3, sc, z));
+                    __stcs(reinterpret_cast<uint2 *>(dst + (i * 8 + 2 * t + e) * HD + 32 * w + 4 * g), o);
+                }
             }
         }
     }

@@ -927,10 +927,21 @@ int paged_limits(int B, int npages, int maxpages) {
     return OUMU_OK;
 }
 
-// 8-warp CTAs of one warp per (take, block of 8 positions, kv head, K or V); 0 where the grid would be too large.
-unsigned kv4_grid(int B, long blocks, int nk) {
-    const long ctas = (static_cast<long>(B) * blocks * 2 * nk + 7) / 8;
-    return ctas <= 0x7fffffffL ? static_cast<unsigned>(ctas) : 0u;
+// How prompt writes and reads are cut: `blocks` blocks of 8 positions of every take in parts of `per`, a warp per part, kv
+// head and K or V, 8 warps a CTA. Parts of one block while the GPU has room for all their warps at once (a prompt of
+// 1024 positions: latency counts), else of 4, whose loads overlap.
+struct Kv4Cut {
+    int per, parts;
+    unsigned grid;  // 0: too large
+};
+Kv4Cut kv4_cut(int B, long blocks, int nk, int sms) {
+    Kv4Cut c;
+    c.per = static_cast<long>(B) * blocks * 2 * nk <= 32L * sms ? 1 : 4;
+    const long parts = (blocks + c.per - 1) / c.per;
+    const long ctas = (B * parts * 2 * nk + 7) / 8;
+    c.parts = static_cast<int>(parts);
+    c.grid = parts < 0x7fffffffL && ctas <= 0x7fffffffL ? static_cast<unsigned>(ctas) : 0u;
+    return c;
 }
 
 size_t kv4_part_bytes(int hd) { return 2 * (2 * static_cast<size_t>(d4::GMAX) + d4::GMAX * hd) * 4; }
@@ -1012,13 +1023,16 @@ int oumu_kv4_write(const void *qkv, void *pool, const int *table, const int *sta
     if (!aligned16(qkv) || !aligned16(pool)) return OUMU_ERR_INVALID;
     if (!start && !count && rows > static_cast<long>(maxpages) * kv4::PAGE) return OUMU_ERR_INVALID;
     if (rows == 0) return OUMU_OK;
-    const int blocks = (rows + 7) / 8 + (start ? 1 : 0);
-    const unsigned grid = kv4_grid(B, blocks, nk);
-    if (!grid) return OUMU_ERR_UNSUPPORTED;
+    int sms = 0;
+    rc = current_device(&sms);
+    if (rc) return rc;
+    // a start inside a part: up to 4 blocks more
+    const Kv4Cut cut = kv4_cut(B, (static_cast<long>(rows) + 7) / 8 + (start ? 4 : 0), nk, sms);
+    if (!cut.grid) return OUMU_ERR_UNSUPPORTED;
     auto kern = hd == 128 ? kv4::k_kv4_write<128> : kv4::k_kv4_write<64>;
-    kern<<<grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(static_cast<const bf16 *>(qkv),
-                                                                   static_cast<uint8_t *>(pool), table, start, count, B,
-                                                                   rows, nq, nk, npages, maxpages, blocks);
+    kern<<<cut.grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+        static_cast<const bf16 *>(qkv), static_cast<uint8_t *>(pool), table, start, count, B, rows, nq, nk, npages,
+        maxpages, cut.parts, cut.per);
     OUMU_CK(cudaGetLastError());
     return OUMU_OK;
 }
@@ -1031,13 +1045,16 @@ int oumu_kv4_read(const void *pool, const int *table, const int *lens, const int
     if (!head_dim_ok(hd)) return OUMU_ERR_UNSUPPORTED;
     if (!aligned16(pool) || !aligned16(kc) || !aligned16(vc)) return OUMU_ERR_INVALID;
     const long span = std::min(static_cast<long>(maxlen), static_cast<long>(maxpages) * kv4::PAGE);
-    const int blocks = static_cast<int>((span + 7) / 8);
-    const unsigned grid = kv4_grid(B, blocks, nk);
-    if (!grid) return OUMU_ERR_UNSUPPORTED;
-    auto kern = hd == 128 ? kv4::k_kv4_read<128> : kv4::k_kv4_read<64>;
-    kern<<<grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+    int sms = 0;
+    rc = current_device(&sms);
+    if (rc) return rc;
+    const Kv4Cut cut = kv4_cut(B, (span + 7) / 8, nk, sms);
+    if (!cut.grid) return OUMU_ERR_UNSUPPORTED;
+    auto kern = hd == 128 ? (cut.per == 1 ? kv4::k_kv4_read<128, 1> : kv4::k_kv4_read<128, 4>)
+                          : (cut.per == 1 ? kv4::k_kv4_read<64, 1> : kv4::k_kv4_read<64, 4>);
+    kern<<<cut.grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
         static_cast<uint8_t *>(const_cast<void *>(pool)), table, lens, pos, static_cast<bf16 *>(kc),
-        static_cast<bf16 *>(vc), B, nk, npages, maxpages, maxlen, blocks);
+        static_cast<bf16 *>(vc), B, nk, npages, maxpages, maxlen, cut.parts);
     OUMU_CK(cudaGetLastError());
     return OUMU_OK;
 }

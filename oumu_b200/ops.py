@@ -17,7 +17,8 @@ def _p(t):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # the current stream's handle without building a Stream object around it (0.3 us a call instead of 3.3)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def rotary_tables(maxlen, hd, ext=None):
