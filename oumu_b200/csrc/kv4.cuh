@@ -132,7 +132,7 @@ __device__ __forceinline__ uint32_t quant_pairs(const uint32_t (&x)[NP], const Q
     const float2 rv = make_float2(q.rinv, q.rinv), ms = make_float2(-q.s, -q.s);
     const float2 mz = make_float2(-q.z, -q.z), mg = make_float2(magic, magic), back = make_float2(-magic, -magic);
     uint32_t lo = 0, hi = 0;
-    float far = 0.f;
+    float far = q.rinv < 1.7e38f ? 0.f : INFINITY;  // no normal reciprocal: a scale of 0 or below 2^-127
     float2 f[NP], d[NP], r[NP];
 #pragma unroll
     for (int i = NP - 1; i >= 0; i--) {
@@ -145,10 +145,9 @@ __device__ __forceinline__ uint32_t quant_pairs(const uint32_t (&x)[NP], const Q
         lo = lo * 16u + __float_as_uint(a.x);  // the magic number's own bits leave the low 16
         hi = hi * 16u + __float_as_uint(a.y);
     }
-    const bool normal = q.rinv < 1.7e38f;  // not for scales of 0 or below 2^-127
-    if (!(far < h && normal)) {
+    if (!(far < h)) {
         // a tie (among bf16 numbers common), or something rarer
-        bool odd = !(far <= h && normal);
+        bool odd = !(far <= h);
 #pragma unroll
         for (int i = 0; i < NP; i++)
             odd = odd || __fadd_rn(d[i].x, q.z) != f[i].x || __fadd_rn(d[i].y, q.z) != f[i].y;
@@ -279,22 +278,42 @@ __global__ void __launch_bounds__(256) k_kv4_write(const bf16 *qkv, uint8_t *poo
                 for (int w = 0; w < W; w++) x[e][w] = y[e][w];
             if (b < last) load(b + 1, y);
             Words<W> code, meta;
+            // ranges of the 2 W groups over the 8 lanes of a position pair: each exchange halves what a lane holds, until
+            // lane g has one group's and works out its scale, which then goes to all
+            uint32_t rg[2 * W];
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int w = 0; w < W; w++)
+                    rg[e * W + w] = range_of(as_u32(__hmax2_nan(as_bf2(x[e][w].x), as_bf2(x[e][w].y))),
+                                             as_u32(__hmin2_nan(as_bf2(x[e][w].x), as_bf2(x[e][w].y))));
+#pragma unroll
+            for (int m = W, o = 16; m >= 1; m >>= 1, o >>= 1) {
+                const bool up = lane & o;
+#pragma unroll
+                for (int i = 0; i < m; i++) {
+                    const uint32_t send = up ? rg[i] : rg[i + m], keep = up ? rg[i + m] : rg[i];
+                    rg[i] = range_max(keep, __shfl_xor_sync(0xffffffffu, send, o));
+                }
+            }
+            if (W == 2) rg[0] = range_max(rg[0], __shfl_xor_sync(0xffffffffu, rg[0], 4));
+            const Quant mine = quant_of(rg[0]);
+            const uint32_t mine_sz = meta_bits(mine.s, mine.z);
             uint32_t sz[2][W];
 #pragma unroll
             for (int w = 0; w < W; w++) {
                 uint32_t n4[2];
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const uint2 v = x[e][w];
-                    uint32_t rg = range_of(as_u32(__hmax2_nan(as_bf2(v.x), as_bf2(v.y))),
-                                           as_u32(__hmin2_nan(as_bf2(v.x), as_bf2(v.y))));
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, o));
-                    const Quant q = quant_of(rg);
-                    const uint32_t pr[2] = {v.x, v.y};
+                    const int from = (e * W + w) * (16 / W) + t;
+                    sz[e][w] = __shfl_sync(0xffffffffu, mine_sz, from);
+                    Quant q;
+                    q.s = __uint_as_float(sz[e][w] << 16);
+                    q.z = __uint_as_float(sz[e][w] & 0xffff0000u);
+                    q.rinv = __shfl_sync(0xffffffffu, mine.rinv, from);
+                    const uint32_t pr[2] = {x[e][w].x, x[e][w].y};
                     const uint32_t c = quant_pairs<2>(pr, q);  // low half: channels 0, 2; high half: 1, 3
                     n4[e] = (c & 0xfu) | (c >> 12 & 0xf0u) | (c << 4 & 0xf00u) | (c >> 8 & 0xf000u);
-                    sz[e][w] = meta_bits(q.s, q.z);
                 }
                 code.v[w] = __byte_perm(n4[0], n4[1], 0x5410);
             }
