@@ -372,15 +372,15 @@ __global__ void __launch_bounds__(256) k_kv4_read(uint8_t *pool, const int *tabl
     if (b0 * 8 >= L) return;
     const uint8_t *u = unit_of(pool, table, it.s, b0 * 8, it.h, nk, npages, maxpages, F::UNIT);
     if (!u) return;
-    u += (b0 & 7) / 4 * F::HALFB;
     bf16 *dst = (it.v ? vc : kc) + ((static_cast<long>(it.s) * nk + it.h) * maxlen + b0 * 8) * HD;
     const int left = L - b0 * 8;
     Words<W> code[PER], m[PER][2];
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         if (i * 8 >= left) break;
-        code[i] = ld_words<W>(u + it.v * F::CODES + ((b0 + i) & 3) * F::BLOCK + lane * 4 * W);
-        const uint8_t *rows = u + (it.v ? F::VMETA : F::KMETA) + ((b0 + i) & 3) * 8 * F::ROW;
+        const uint8_t *half = u + ((b0 + i) & 7) / 4 * F::HALFB;
+        code[i] = ld_words<W>(half + it.v * F::CODES + ((b0 + i) & 3) * F::BLOCK + lane * 4 * W);
+        const uint8_t *rows = half + (it.v ? F::VMETA : F::KMETA) + ((b0 + i) & 3) * 8 * F::ROW;
         m[i][0] = ld_words<W>(rows + (it.v ? 2 * t : g) * F::ROW);
         if (it.v) m[i][1] = ld_words<W>(rows + (2 * t + 1) * F::ROW);
     }
