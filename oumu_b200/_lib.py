@@ -62,6 +62,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_fns = {}  # entry points by name
 
 
 class OumuError(RuntimeError):
@@ -87,6 +88,7 @@ def load():
             f = getattr(lib, name)
             f.restype = res
             f.argtypes = args
+            _fns[name] = f
         _lib = lib
     return _lib
 
@@ -103,6 +105,7 @@ CALLS = [0]
 def call(name, *args):
     """Call entry point `name` and raise OumuError on a non-zero status."""
     CALLS[0] += 1
-    st = getattr(load(), name)(*args)
-    check(name, st)
+    st = (_fns.get(name) or getattr(load(), name))(*args)
+    if st != OK:
+        raise OumuError(name, st)
     return st

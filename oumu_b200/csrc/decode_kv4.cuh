@@ -532,6 +532,10 @@ constexpr int ST = 4;           // tiles in flight per warp: 8 x 4 x 5 KB = 160 
 constexpr int NT = NW * 32;
 static_assert(NW <= 16, "a half warp holds a reference per warp");
 constexpr int MIN_TILES = 2 * NW;  // tiles per CTA at least
+// CTA boundaries do not cut segments of up to so many tiles, three per warp (hd 128): adding up records across CTAs costs
+// about 3 us, as long as a CTA's work growing by that many tiles.
+template <int HD>
+constexpr int SNAP = 3 * NW * (128 / HD);
 
 // A segment that crosses a boundary: take * nk + kv head, its tiles, the CTA's warps that have some of them.
 struct Cross {
@@ -651,7 +655,18 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
     const int want = (W + MIN_TILES - 1) / MIN_TILES, Gc = want < static_cast<int>(gridDim.x) ? want : gridDim.x;
     if (c >= Gc) return;
     const Parts ctas(W, Gc);
-    const int ta = ctas.start(c), tb = ctas.start(c + 1);
+    int ta, tb;
+    {
+        // a boundary inside a short segment moves to the segment's nearer end: lanes 0 and 1 find this CTA's two
+        int t = ctas.start(min(c + (lane & 1), Gc));
+        if (t < W) {
+            const int s = take_of(pre, B, t), T = tiles_of(Ls[s]), j = (t - pre[s]) % T;
+            if (T <= SNAP<HD>) t += 2 * j < T ? -j : T - j;
+        }
+        ta = __shfl_sync(0xffffffffu, t, 0);
+        tb = __shfl_sync(0xffffffffu, t, 1);
+    }
+    if (ta >= tb) return;
     const Parts parts(tb - ta, NW);
     const int wa = ta + parts.start(warp), wb = ta + parts.start(warp + 1), n = wb - wa;
 
