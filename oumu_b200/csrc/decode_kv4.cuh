@@ -521,35 +521,43 @@ struct Newest {
     }
 };
 
-// Work is counted in tiles (halves of 32 positions of one take and kv head, a "segment"), laid end to end take by take
-// and cut into equal contiguous ranges: one per CTA, and that into one per warp. A warp streams its range through a
-// ring of its own in shared memory (one bulk copy of 5 KB per tile, nothing shared, no producer warp), so a CTA keeps
-// NW * ST copies in flight and no warp waits for another before the range's end. A segment that lies inside a warp's
-// range is finished by it alone; the parts of one that crosses warps meet in shared memory, of one that crosses CTAs in
-// records in global memory, where the last to arrive adds them up in CTA order: the result does not depend on timing.
-constexpr int NW = 8;           // warps
-constexpr int ST = 4;           // tiles in flight per warp: 8 x 4 x 5 KB = 160 KB per SM
-constexpr int NT = NW * 32;
-static_assert(NW <= 16, "a half warp holds a reference per warp");
-constexpr int MIN_TILES = 2 * NW;  // tiles per CTA at least
-// CTA boundaries do not cut segments of up to so many tiles, three per warp (hd 128): adding up records across CTAs costs
-// about 3 us, as long as a CTA's work growing by that many tiles.
+// Work is counted in tiles (5 KB: 32 positions of one take and kv head, a "segment", at hd 128, 64 at hd 64), laid end to
+// end take by take and cut into equal contiguous ranges: one per CTA, and that into one per warp. A warp streams its range
+// through a ring of its own in shared memory (one bulk copy per tile, nothing shared, no producer warp), so no warp waits
+// for another before the range's end. A segment that lies inside a warp's range is finished by it alone; the parts of one
+// that crosses warps meet in shared memory, of one that crosses CTAs in records in global memory, where the last to arrive
+// adds them up in CTA order: the result does not depend on timing.
+//
+// NW warps and ST tiles in flight for each. 12 warps keep three per scheduler, which hides more of the instructions'
+// latencies (5 KB of cache take about 650 instructions): 6.2 TB/s on long caches against 5.4 with 8 (of 7.1 for the
+// copies alone). 8 warps have less to merge at the end: one take of 512 positions 7.6 us against 8.4.
 template <int HD>
-constexpr int SNAP = 3 * NW * (128 / HD);
+constexpr int TP = HD == 128 ? kv4::HALF : kv4::PAGE;  // positions per tile
+template <int NW>
+constexpr int ST = NW == 8 ? 4 : 2;
+// tiles per CTA at least
+template <int NW>
+constexpr int MIN_TILES = 2 * NW;
+// CTA boundaries do not cut segments of up to so many tiles, three per warp: adding up records across CTAs costs about
+// 3 us, as long as a CTA's work growing by that many tiles.
+template <int NW>
+constexpr int SNAP = 3 * NW;
 
 // A segment that crosses a boundary: take * nk + kv head, its tiles, the CTA's warps that have some of them.
 struct Cross {
     int id, start, end, first, last;
 };
 
-template <int HD>
+template <int HD, int NW>
 struct Lay {
+    static_assert(NW <= 16, "a half warp holds a reference per warp");
     static constexpr int REC = 2 * GMAX + GMAX * HD;  // floats of a record: m[8], l[8], o[8][HD]
-    static_assert(REC * 4 <= ST * Fmt<HD>::HALFB, "a warp's last record lies in its own ring");
-    static constexpr int RING = ST * Fmt<HD>::HALFB;
+    static constexpr int TILE = TP<HD> / kv4::HALF * Fmt<HD>::HALFB;
+    static constexpr int RING = ST<NW> * TILE;
+    static_assert(REC * 4 <= RING, "a warp's last record lies in its own ring");
     static constexpr int FIRST = NW * RING;           // records of segments that end inside a warp's range
     static constexpr int BAR = FIRST + NW * REC * 4;
-    static constexpr int LIST = BAR + NW * ST * 8;    // segments that cross warps
+    static constexpr int LIST = BAR + NW * ST<NW> * 8;    // segments that cross warps
     static constexpr int MISC = LIST + (NW + 1) * static_cast<int>(sizeof(Cross));
     static constexpr int PRE = MISC + 128;            // pre[B + 1], lens[B]
     static __host__ __device__ int bytes(int B) { return PRE + (2 * B + 1) * 4; }
@@ -576,7 +584,8 @@ __device__ __forceinline__ int take_len(const Params &P, int s) {
     }
     return L;
 }
-__device__ __forceinline__ int tiles_of(int L) { return (L + HALF - 1) / HALF; }
+template <int HD>
+__device__ __forceinline__ int tiles_of(int L) { return (L + TP<HD> - 1) / TP<HD>; }
 
 // The take whose tiles hold tile t: the last s with pre[s] <= t (takes without tiles are passed over).
 __device__ __forceinline__ int take_of(const int *pre, int B, int t) {
@@ -598,10 +607,11 @@ struct Parts {
     }
 };
 
-template <int HD, bool FUSED>
-__global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
+template <int HD, int NW, bool FUSED>
+__global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
     using F = Fmt<HD>;
-    using Y = Lay<HD>;
+    using Y = Lay<HD, NW>;
+    constexpr int NT = NW * 32, ST = d4::ST<NW>, TP = d4::TP<HD>;
     extern __shared__ __align__(128) uint8_t sm[];
     int *pre = reinterpret_cast<int *>(sm + Y::PRE), *Ls = pre + P.B + 1;
     int *misc = reinterpret_cast<int *>(sm + Y::MISC);
@@ -617,7 +627,7 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
     {
         int run = 0;
         for (int s0 = 0; s0 < B; s0 += NT) {
-            const int s = s0 + threadIdx.x, L = s < B ? take_len(P, s) : 0, n = tiles_of(L) * nk;
+            const int s = s0 + threadIdx.x, L = s < B ? take_len(P, s) : 0, n = tiles_of<HD>(L) * nk;
             int x = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -652,7 +662,7 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
             for (int i = threadIdx.x; i < 2 * nk * HD / 8; i += NT)
                 reinterpret_cast<uint4 *>(P.held + static_cast<long>(s) * 2 * nk * HD)[i] = zero;
     }
-    const int want = (W + MIN_TILES - 1) / MIN_TILES, Gc = want < static_cast<int>(gridDim.x) ? want : gridDim.x;
+    const int want = (W + MIN_TILES<NW> - 1) / MIN_TILES<NW>, Gc = want < static_cast<int>(gridDim.x) ? want : gridDim.x;
     if (c >= Gc) return;
     const Parts ctas(W, Gc);
     int ta, tb;
@@ -660,8 +670,8 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
         // a boundary inside a short segment moves to the segment's nearer end: lanes 0 and 1 find this CTA's two
         int t = ctas.start(min(c + (lane & 1), Gc));
         if (t < W) {
-            const int s = take_of(pre, B, t), T = tiles_of(Ls[s]), j = (t - pre[s]) % T;
-            if (T <= SNAP<HD>) t += 2 * j < T ? -j : T - j;
+            const int s = take_of(pre, B, t), T = tiles_of<HD>(Ls[s]), j = (t - pre[s]) % T;
+            if (T <= SNAP<NW>) t += 2 * j < T ? -j : T - j;
         }
         ta = __shfl_sync(0xffffffffu, t, 0);
         tb = __shfl_sync(0xffffffffu, t, 1);
@@ -679,7 +689,7 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
         const bool any = lane < NW ? at < tb : lane == NW;  // a warp without tiles starts where the CTA ends
         if (any) {
             // the segment of tile `at`, at the CTA's end of the tile before: its start is known to the warp that has it
-            const int s = take_of(pre, B, lane < NW ? at : tb - 1), T = tiles_of(Ls[s]);
+            const int s = take_of(pre, B, lane < NW ? at : tb - 1), T = tiles_of<HD>(Ls[s]);
             const int kh = ((lane < NW ? at : tb - 1) - pre[s]) / T;
             x.id = s * nk + kh;
             x.start = pre[s] + kh * T;
@@ -702,22 +712,23 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
         auto look_up = [&](int base) {
             const int t = wa + base + lane;
             if (t >= wb) return;
-            const int s = take_of(pre, B, t), T = tiles_of(Ls[s]), off = t - pre[s], kh = off / T, j = off - kh * T;
-            int page = P.table[static_cast<long>(s) * P.maxpages + j / 2];
+            const int s = take_of(pre, B, t), T = tiles_of<HD>(Ls[s]), off = t - pre[s], kh = off / T, j = off - kh * T;
+            constexpr int per = kv4::PAGE / TP;  // tiles of a page
+            int page = P.table[static_cast<long>(s) * P.maxpages + j / per];
             if (page < 0 || page >= P.npages) {
                 record_error(OUMU_DEVERR_PAGE);
                 page = 0;  // read in its place: the take's output is unspecified
             }
-            src = P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + (j & 1) * F::HALFB;
+            src = P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + j % per * Y::TILE;
         };
         auto issue = [&](int k) {  // tile k into its stage
             const unsigned long long a = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k & 31);
-            bulk_load_first_lane(ring + (k % ST) * F::HALFB, a, F::HALFB, bars + 8 * (k % ST), lane);
+            bulk_load_first_lane(ring + (k % ST) * Y::TILE, a, Y::TILE, bars + 8 * (k % ST), lane);
         };
         look_up(0);
         issue(0);
         if (warp == 0) list_crossings();  // while the first copies are on their way
-        int s = take_of(pre, B, wa), T = tiles_of(Ls[s]), kh = (wa - pre[s]) / T, j = wa - pre[s] - kh * T;
+        int s = take_of(pre, B, wa), T = tiles_of<HD>(Ls[s]), kh = (wa - pre[s]) / T, j = wa - pre[s] - kh * T;
         int k = 0, issued = 1;
         while (k < n) {
             // ---- this warp's part of a segment: tiles j .. of take s, kv head kh ----
@@ -729,25 +740,26 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
             S.clear();
             const bool ends = stop == k + T - j;  // its last tile is this warp's
             if (FUSED && ends) {
-                const int page = P.table[static_cast<long>(s) * P.maxpages + (T - 1) / 2];
+                const int page = P.table[static_cast<long>(s) * P.maxpages + (L - 1) / kv4::PAGE];
                 if (page >= 0 && page < P.npages)
                     N.make(P, s, kh, L - 1, lane,
-                           P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + ((T - 1) & 1) * F::HALFB);
+                           P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + (L - 1) % kv4::PAGE / HALF * F::HALFB);
             }
             for (; issued < ST && issued < n; issued++) issue(issued);  // behind every warp's first tile
-            int left = L - j * HALF;  // positions from this tile on
-            for (; k < stop; k++, left -= HALF) {
+            int left = L - j * TP;  // positions from this tile on
+            for (; k < stop; k++, left -= TP) {
                 const uint32_t bar = bars + 8 * (k % ST), phase = (k / ST) & 1;
                 if (!__all_sync(0xffffffffu, mbar_try_wait(bar, phase)) &&
                     !__all_sync(0xffffffffu, mbar_wait(bar, phase)))
                     break;
-                uint8_t *half = sm + warp * Y::RING + (k % ST) * F::HALFB;
+                uint8_t *half = sm + warp * Y::RING + (k % ST) * Y::TILE;
                 if (FUSED && ends && k == stop - 1) {
-                    N.patch(half, (L - 1) % HALF, lane);
+                    N.patch(half + (L - 1) % TP / HALF * F::HALFB, (L - 1) % HALF, lane);
                     fence_proxy_async_smem();  // before the stage's next copy
                     __syncwarp();
                 }
-                S.tile(half, left, Q, lane);
+#pragma unroll 1
+                for (int h = 0; h < TP / HALF && left > h * HALF; h++) S.tile(half + h * F::HALFB, left - h * HALF, Q, lane);
                 __syncwarp();
                 if (issued < n) {
                     if ((issued & 31) == 0) look_up(issued);
@@ -771,7 +783,7 @@ __global__ void __launch_bounds__(NT, 1) k_attn_decode_kv4(Params P) {
             if (++kh == nk) {
                 kh = 0;
                 do ++s; while (s < B && Ls[s] == 0);
-                T = s < B ? tiles_of(Ls[s]) : 1;
+                T = s < B ? tiles_of<HD>(Ls[s]) : 1;
             }
         }
     }

@@ -142,8 +142,10 @@ int current_device(int *sms) {
                                      kSmemMax));
         OUMU_CK(cudaFuncSetAttribute(gm::k_gemm<128, kGemmStages128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      kSmemMax));
-        for (auto kern : {d4::k_attn_decode_kv4<128, false>, d4::k_attn_decode_kv4<128, true>,
-                          d4::k_attn_decode_kv4<64, false>, d4::k_attn_decode_kv4<64, true>})
+        for (auto kern : {d4::k_attn_decode_kv4<128, 8, false>, d4::k_attn_decode_kv4<128, 8, true>,
+                          d4::k_attn_decode_kv4<128, 12, false>, d4::k_attn_decode_kv4<128, 12, true>,
+                          d4::k_attn_decode_kv4<64, 8, false>, d4::k_attn_decode_kv4<64, 8, true>,
+                          d4::k_attn_decode_kv4<64, 12, false>, d4::k_attn_decode_kv4<64, 12, true>})
             OUMU_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
         di.ready = true;
     }
@@ -955,13 +957,21 @@ Kv4Cut kv4_cut(int B, long blocks, int nk, int sms, int large) {
 
 size_t kv4_part_bytes(int hd) { return 2 * (2 * static_cast<size_t>(d4::GMAX) + d4::GMAX * hd) * 4; }
 
-template <int HD, bool FUSED>
-int launch_decode_kv4(const d4::Params &P, size_t ws_bytes, int sms, cudaStream_t st) {
+template <int HD, int NW>
+int launch_decode_kv4(bool fused, const d4::Params &P, size_t ws_bytes, int sms, cudaStream_t st) {
     // one CTA per SM, fewer where the workspace holds fewer CTAs' records
     const long fit = static_cast<long>((ws_bytes - decode_counter_bytes(P.B, P.nk)) / kv4_part_bytes(HD));
     const unsigned grid = static_cast<unsigned>(std::min(static_cast<long>(sms), fit));
-    OUMU_CK(launch_k(d4::k_attn_decode_kv4<HD, FUSED>, dim3(grid), dim3(d4::NT), d4::Lay<HD>::bytes(P.B), st, P));
+    OUMU_CK(launch_k(fused ? d4::k_attn_decode_kv4<HD, NW, true> : d4::k_attn_decode_kv4<HD, NW, false>, dim3(grid),
+                     dim3(NW * 32), d4::Lay<HD, NW>::bytes(P.B), st, P));
     return OUMU_OK;
+}
+// 12 warps where full tables would give 8 warps an SM 16 tiles each, or more (lengths are known on the device only).
+template <int HD>
+int launch_decode_kv4(bool fused, const d4::Params &P, size_t ws_bytes, int sms, cudaStream_t st) {
+    const long tiles = static_cast<long>(P.B) * P.nk * P.maxpages * (kv4::PAGE / d4::TP<HD>);
+    return tiles >= 16L * 8 * sms ? launch_decode_kv4<HD, 12>(fused, P, ws_bytes, sms, st)
+                                  : launch_decode_kv4<HD, 8>(fused, P, ws_bytes, sms, st);
 }
 
 int decode_kv4_entry(bool fused, const void *qkv, void *pool, void *out, void *held, void *ws, size_t ws_bytes,
@@ -1001,11 +1011,8 @@ int decode_kv4_entry(bool fused, const void *qkv, void *pool, void *out, void *h
     P.maxpages = maxpages;
     P.sl2 = scale * 1.4426950408889634f;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (fused)
-        return hd == 128 ? launch_decode_kv4<128, true>(P, ws_bytes, sms, st)
-                         : launch_decode_kv4<64, true>(P, ws_bytes, sms, st);
-    return hd == 128 ? launch_decode_kv4<128, false>(P, ws_bytes, sms, st)
-                     : launch_decode_kv4<64, false>(P, ws_bytes, sms, st);
+    return hd == 128 ? launch_decode_kv4<128>(fused, P, ws_bytes, sms, st)
+                     : launch_decode_kv4<64>(fused, P, ws_bytes, sms, st);
 }
 
 // Pools of `layers` layers; layer_stride only matters from the second on.
