@@ -535,9 +535,9 @@ template <int HD>
 constexpr int TP = HD == 128 ? kv4::HALF : kv4::PAGE;  // positions per tile
 template <int NW>
 constexpr int ST = NW == 8 ? 4 : 2;
-// tiles per CTA at least
+// tiles per CTA at least: one a warp
 template <int NW>
-constexpr int MIN_TILES = 2 * NW;
+constexpr int MIN_TILES = NW;
 // CTA boundaries do not cut segments of up to so many tiles, three per warp: adding up records across CTAs costs about
 // 3 us, as long as a CTA's work growing by that many tiles.
 template <int NW>
@@ -622,7 +622,6 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
     if (lane < ST) mbar_init(bars + 8 * lane, 1);
     mbar_fence_init();
     pdl_trigger();
-    pdl_wait();
     // tiles before every take
     {
         int run = 0;
@@ -653,20 +652,10 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
     }
     __syncthreads();
     const int W = pre[B];
-    for (int s = c; s < B; s += gridDim.x) {  // takes that hold nothing
-        if (Ls[s] > 0) continue;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        for (int i = threadIdx.x; i < P.nq * HD / 8; i += NT)
-            reinterpret_cast<uint4 *>(P.out + static_cast<long>(s) * P.nq * HD)[i] = zero;
-        if (FUSED && P.held)
-            for (int i = threadIdx.x; i < 2 * nk * HD / 8; i += NT)
-                reinterpret_cast<uint4 *>(P.held + static_cast<long>(s) * 2 * nk * HD)[i] = zero;
-    }
     const int want = (W + MIN_TILES<NW> - 1) / MIN_TILES<NW>, Gc = want < static_cast<int>(gridDim.x) ? want : gridDim.x;
-    if (c >= Gc) return;
-    const Parts ctas(W, Gc);
-    int ta, tb;
-    {
+    int ta = 0, tb = 0;
+    const Parts ctas(W, Gc > 0 ? Gc : 1);
+    if (c < Gc) {
         // a boundary inside a short segment moves to the segment's nearer end: lanes 0 and 1 find this CTA's two
         int t = ctas.start(min(c + (lane & 1), Gc));
         if (t < W) {
@@ -676,7 +665,22 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         ta = __shfl_sync(0xffffffffu, t, 0);
         tb = __shfl_sync(0xffffffffu, t, 1);
     }
-    if (ta >= tb) return;
+    auto after_predecessor = [&] {  // what the preceding kernel may write is read, and memory written, from here on
+        pdl_wait();
+        for (int s = c; s < B; s += gridDim.x) {  // takes that hold nothing
+            if (Ls[s] > 0) continue;
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            for (int i = threadIdx.x; i < P.nq * HD / 8; i += NT)
+                reinterpret_cast<uint4 *>(P.out + static_cast<long>(s) * P.nq * HD)[i] = zero;
+            if (FUSED && P.held)
+                for (int i = threadIdx.x; i < 2 * nk * HD / 8; i += NT)
+                    reinterpret_cast<uint4 *>(P.held + static_cast<long>(s) * 2 * nk * HD)[i] = zero;
+        }
+    };
+    if (ta >= tb) {
+        after_predecessor();
+        return;
+    }
     const Parts parts(tb - ta, NW);
     const int wa = ta + parts.start(warp), wb = ta + parts.start(warp + 1), n = wb - wa;
 
@@ -725,9 +729,13 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
             const unsigned long long a = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k & 31);
             bulk_load_first_lane(ring + (k % ST) * Y::TILE, a, Y::TILE, bars + 8 * (k % ST), lane);
         };
+        // Fused, a copy may come before the preceding kernel's end: that kernel writes no page, and the newest position is
+        // patched in. Otherwise it may be the write of the newest position.
+        if (!FUSED) after_predecessor();
         look_up(0);
         issue(0);
         if (warp == 0) list_crossings();  // while the first copies are on their way
+        if (FUSED) after_predecessor();
         int s = take_of(pre, B, wa), T = tiles_of<HD>(Ls[s]), kh = (wa - pre[s]) / T, j = wa - pre[s] - kh * T;
         int k = 0, issued = 1;
         while (k < n) {
@@ -786,6 +794,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
                 T = s < B ? tiles_of<HD>(Ls[s]) : 1;
             }
         }
+    } else {
+        after_predecessor();
     }
     __syncthreads();
 
@@ -863,30 +873,44 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         if (!(crossing >> k & 1) || !misc[1 + k] || h >= G) continue;
         const Cross x = list[k ? nlist - 1 : 0];
         const int cf = ctas.of(x.start), cl = ctas.of(x.end - 1);
-        auto at = [&](int cc) { return P.part + (static_cast<long>(cc) * 2 + (cc == cf)) * Y::REC; };
-        // the head's LPH threads take a record's reference each
-        float M = -INFINITY, l = 0.f;
+        auto at = [&](int cc) { return P.part + (static_cast<long>(cc) * 2 + (cc == cf)) * Y::REC + h; };
+        auto numer = [&](int cc) {
+            return __ldcg(reinterpret_cast<const float4 *>(at(cc) - h + 2 * GMAX + h * HD + 4 * d4));
+        };
+        // up to 16 records' numerators on their way while the head's LPH threads take a record's reference and sum each
+        constexpr int N = 16;
+        const unsigned mates = LPH == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
+        float4 v[N];
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] = cf + e <= cl ? numer(cf + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+        float m = cf + d4 <= cl ? __ldcg(at(cf + d4)) : -INFINITY;
+        float lw = cf + d4 <= cl ? __ldcg(at(cf + d4) + GMAX) : 0.f;
+        float M = m, l = 0.f;
+        for (int cc = cf + d4 + LPH; cc <= cl; cc += LPH) M = fmaxf(M, __ldcg(at(cc)));
+#pragma unroll
+        for (int e = 1; e < LPH; e <<= 1) M = fmaxf(M, __shfl_xor_sync(mates, M, e, LPH));  // a head's threads come together
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float f = fast_exp2(m - M);
+        l = f * lw;
 #pragma unroll 1
-        for (int cc = cf + d4; cc <= cl; cc += LPH) M = fmaxf(M, __ldcg(at(cc) + h));
+        for (int c0 = cf;;) {
 #pragma unroll
-        for (int e = 1; e < LPH; e <<= 1)  // a head's threads come here together
-            M = fmaxf(M, __shfl_xor_sync(LPH == 32 ? 0xffffffffu : 0xffffu << (lane & 16), M, e, LPH));
-#pragma unroll 1
-        for (int c0 = cf; c0 <= cl; c0 += 8) {
-            float m[8], lw[8];
-            float4 v[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float *R = at(min(c0 + e, cl));
-                m[e] = __ldcg(R + h);
-                lw[e] = __ldcg(R + GMAX + h);
-                v[e] = __ldcg(reinterpret_cast<const float4 *>(R + 2 * GMAX + h * HD + 4 * d4));
+            for (int e = 0; e < N; e++) {
+                const float fe = __shfl_sync(mates, f, (c0 - cf + e) % LPH, LPH);
+                o = make_float4(fmaf(fe, v[e].x, o.x), fmaf(fe, v[e].y, o.y), fmaf(fe, v[e].z, o.z), fmaf(fe, v[e].w, o.w));
             }
+            c0 += N;
+            if (c0 > cl) break;
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (c0 + e <= cl) add(fast_exp2(m[e] - M), lw[e], v[e], l, o);
+            for (int e = 0; e < N; e++) v[e] = c0 + e <= cl ? numer(c0 + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            if ((c0 - cf) % LPH == 0) {  // the next LPH records' references
+                const bool in = c0 + d4 <= cl;
+                f = in ? fast_exp2(__ldcg(at(c0 + d4)) - M) : 0.f;
+                l = in ? fmaf(f, __ldcg(at(c0 + d4) + GMAX), l) : l;
+            }
         }
+#pragma unroll
+        for (int e = 1; e < LPH; e <<= 1) l += __shfl_xor_sync(mates, l, e, LPH);
         store(x.id, l, o);
     }
 }
