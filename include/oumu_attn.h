@@ -42,7 +42,8 @@ const char *oumu_last_cuda_error(void);
 
 /*
  * Programmatic dependent launch, process-wide, off by default; returns the previous setting. Applies to the decode
- * kernels (oumu_decode_prologue, oumu_attn_decode, oumu_attn_decode_step), oumu_gemm, the glue kernels
+ * kernels (oumu_decode_prologue, oumu_attn_decode, oumu_attn_decode_step, oumu_attn_decode_kv4,
+ * oumu_attn_decode_kv4_step), oumu_gemm, the glue kernels
  * oumu_rmsnorm, oumu_silu_mul and oumu_pointwise (include/oumu_step.h), and the tensor-memory attention kernels of
  * oumu_attn_full, oumu_attn_full_rope and oumu_attn_prefill_kv (causal prefill, short sequences). When on, these
  * kernels are launched so that they may start while the preceding kernel in the stream is still running: their
@@ -51,7 +52,8 @@ const char *oumu_last_cuda_error(void);
  * and every global write made, only after it has completed. Most let their successor start at once; the attention
  * kernels that hold all of an SM's tensor memory take it only after the preceding kernel has completed and let
  * their successor in only once they hold it. The caller guarantees that the preceding kernels
- * of the same step do not write `pos`/`lens`, cache positions below the newest one, or weights (true of the
+ * of the same step do not write `pos`/`lens`, cache positions below the newest one, or weights, and that a kernel
+ * launched in the ordinary way lies between a call of oumu_pages_* and a decode over its page table (true of the
  * reference's step, where ctr advances only in step_end, src/model.rs:771, and kv_write writes only position *pos,
  * src/model.rs:590-595). Captured into CUDA graphs as programmatic edges.
  */
@@ -256,15 +258,15 @@ int oumu_attn_decode_kv4(const void *qkv, const void *pool, void *out, void *wor
 
 /*
  * oumu_attn_decode_step over the 4-bit cache: in one launch, every take's newest position (lens[s] - 1, or *pos) has
- * its k rotated (cos_t, sin_t [>= that position + 1][hd / 2]; NULL for no rope), k and v quantised into its page, and
- * its q rotated and attended over positions up to and including it, all as the cache stands for them: the output of
+ * its k rotated (cos_t, sin_t [rot_rows][hd / 2]; NULL for no rope; a length above rot_rows is one the table does
+ * not hold), k and v quantised into its page, and its q rotated and attended over positions up to and including it, all as the cache stands for them: the output of
  * oumu_rope, oumu_kv4_write and oumu_attn_decode_kv4, bit for bit. qkv is not modified. held: bf16 [B][2 nk hd] or
  * NULL, receives what the cache now holds of the newest k (heads), then v; zeros for a take of length 0.
  */
 int oumu_attn_decode_kv4_step(const void *qkv, void *pool, void *out, void *held, void *workspace,
-                              size_t workspace_bytes, const float *cos_t, const float *sin_t, const int *table,
-                              const int *pos, const int *lens, int B, int nq, int nk, int hd, int npages,
-                              int maxpages, float scale, oumu_stream_t stream);
+                              size_t workspace_bytes, const float *cos_t, const float *sin_t, int rot_rows,
+                              const int *table, const int *pos, const int *lens, int B, int nq, int nk, int hd,
+                              int npages, int maxpages, float scale, oumu_stream_t stream);
 
 /*
  * Pages of a cache, for any contents: the pool of layer l is `pools` + l * layer_stride, npages pages of page_bytes

@@ -38,7 +38,7 @@ SIGNATURES = {
     "oumu_kv4_read": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "oumu_attn_decode_kv4_workspace": (_Z, [_I, _I, _I, _I, _I]),
     "oumu_attn_decode_kv4": (_I, [_P, _P, _P, _P, _Z, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
-    "oumu_attn_decode_kv4_step": (_I, [_P, _P, _P, _P, _P, _Z, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
+    "oumu_attn_decode_kv4_step": (_I, [_P, _P, _P, _P, _P, _Z, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "oumu_pages_extend": (_I, [_P, _P, _P, _I, _P, _I, _I, _I, _P]),
     "oumu_pages_fork": (_I, [_P, _L, _I, _L, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
     "oumu_pages_free": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P]),

@@ -92,6 +92,7 @@ struct Params {
     int *cnt;                    // [B * nk], zero between launches
     const int *pos, *lens;
     const float *cos_t, *sin_t;  // fused form: rotary tables, or null (no rope)
+    int rot_rows;                // rows of cos_t and sin_t
     int B, nq, nk, npages, maxpages;
     float sl2;                   // scale * log2(e)
 };
@@ -574,10 +575,11 @@ __device__ __forceinline__ void bulk_load_first_lane(uint32_t dst, unsigned long
         : "memory");
 }
 
-// Take s's length: lens[s] or *pos + 1, cut to what its table row can hold (recorded).
+// Take s's length: lens[s] or *pos + 1, cut to what its table row, and the rotary tables, can hold (recorded).
 __device__ __forceinline__ int take_len(const Params &P, int s) {
     int L = P.lens ? P.lens[s] : *P.pos + 1;
-    const int room = P.maxpages * kv4::PAGE;
+    int room = P.maxpages * kv4::PAGE;
+    if (P.cos_t) room = min(room, P.rot_rows);
     if (L < 0 || L > room) {
         record_error(OUMU_DEVERR_LENGTH);
         L = L < 0 ? 0 : room;

@@ -975,11 +975,12 @@ int launch_decode_kv4(bool fused, const d4::Params &P, size_t ws_bytes, int sms,
 }
 
 int decode_kv4_entry(bool fused, const void *qkv, void *pool, void *out, void *held, void *ws, size_t ws_bytes,
-                     const float *cos_t, const float *sin_t, const int *table, const int *pos, const int *lens, int B,
-                     int nq, int nk, int hd, int npages, int maxpages, float scale, oumu_stream_t stream) {
+                     const float *cos_t, const float *sin_t, int rot_rows, const int *table, const int *pos,
+                     const int *lens, int B, int nq, int nk, int hd, int npages, int maxpages, float scale,
+                     oumu_stream_t stream) {
     if (!qkv || !pool || !out || !ws || !table || (!pos && !lens)) return OUMU_ERR_INVALID;
     if (nq < 1 || nk < 1 || nq % nk || !(scale > 0.f)) return OUMU_ERR_INVALID;
-    if ((cos_t == nullptr) != (sin_t == nullptr)) return OUMU_ERR_INVALID;
+    if ((cos_t == nullptr) != (sin_t == nullptr) || (cos_t && rot_rows < 1)) return OUMU_ERR_INVALID;
     int rc = paged_limits(B, npages, maxpages);
     if (rc) return rc;
     if (!head_dim_ok(hd) || nq / nk > d4::GMAX) return OUMU_ERR_UNSUPPORTED;
@@ -1004,6 +1005,7 @@ int decode_kv4_entry(bool fused, const void *qkv, void *pool, void *out, void *h
     P.lens = lens;
     P.cos_t = cos_t;
     P.sin_t = sin_t;
+    P.rot_rows = rot_rows;
     P.B = B;
     P.nq = nq;
     P.nk = nk;
@@ -1086,15 +1088,15 @@ int oumu_attn_decode_kv4(const void *qkv, const void *pool, void *out, void *wor
                          const int *table, const int *pos, const int *lens, int B, int nq, int nk, int hd, int npages,
                          int maxpages, float scale, oumu_stream_t stream) {
     return decode_kv4_entry(false, qkv, const_cast<void *>(pool), out, nullptr, workspace, workspace_bytes, nullptr,
-                            nullptr, table, pos, lens, B, nq, nk, hd, npages, maxpages, scale, stream);
+                            nullptr, 0, table, pos, lens, B, nq, nk, hd, npages, maxpages, scale, stream);
 }
 
 int oumu_attn_decode_kv4_step(const void *qkv, void *pool, void *out, void *held, void *workspace,
-                              size_t workspace_bytes, const float *cos_t, const float *sin_t, const int *table,
-                              const int *pos, const int *lens, int B, int nq, int nk, int hd, int npages,
-                              int maxpages, float scale, oumu_stream_t stream) {
-    return decode_kv4_entry(true, qkv, pool, out, held, workspace, workspace_bytes, cos_t, sin_t, table, pos, lens, B,
-                            nq, nk, hd, npages, maxpages, scale, stream);
+                              size_t workspace_bytes, const float *cos_t, const float *sin_t, int rot_rows,
+                              const int *table, const int *pos, const int *lens, int B, int nq, int nk, int hd,
+                              int npages, int maxpages, float scale, oumu_stream_t stream) {
+    return decode_kv4_entry(true, qkv, pool, out, held, workspace, workspace_bytes, cos_t, sin_t, rot_rows, table, pos,
+                            lens, B, nq, nk, hd, npages, maxpages, scale, stream);
 }
 
 int oumu_pages_extend(int *table, int *ref, const int *lens, int extra, int *status, int B, int npages, int maxpages,

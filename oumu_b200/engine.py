@@ -4,11 +4,12 @@ A host-side restatement of the reference engine's per-step launch sequence, `Eng
 DiT passes with classifier-free guidance (src/model.rs:733-749) -> local encoder on the new patch (:751) -> stop
 head (:754-756) -> base LM step (:758) -> FSQ -> fusion -> residual LM step (:759-764) -> step end (:766-772).
 Every kernel outside the GEMMs is this library's, through the C ABI: the fused decode layer of the LMs
-(oumu_attn_decode_step), the small-sequence attention of the DiT and the local encoder (oumu_attn_full) with its
-rope, and the step glue of include/oumu_step.h. The LM projections (qkv, o, gate|up, down at 1 row per take) run
-on this library's tcgen05 GEMM (oumu_gemm); the DiT's and the heads' GEMMs are cuBLAS through torch (bf16 in and
-out, fp32 accumulate, bias added in the epilogue and rounded once, as the reference's gemm_ex with beta = 1 over a
-bias-filled output, src/gpu.rs:186-229, kernels/voxcpm.cu:70-76).
+(oumu_attn_decode_step, or with kv="int4" oumu_attn_decode_kv4_step over the 4-bit paged cache), the small-sequence
+attention of the DiT and the local encoder (oumu_attn_full) with its rope, and the step glue of include/oumu_step.h.
+The LM projections (qkv, o, gate|up, down at 1 row per take) run on this library's tcgen05 GEMM (oumu_gemm); the
+DiT's and the heads' GEMMs are cuBLAS through torch (bf16 in and out, fp32 accumulate, bias added in the epilogue and
+rounded once, as the reference's gemm_ex with beta = 1 over a bias-filled output, src/gpu.rs:186-229,
+kernels/voxcpm.cu:70-76).
 
 Weights are random (seeded N(0, 0.02) bf16; norm weights 1 + N(0, 0.02)) and the KV slots hold random prompt
 state: the step is for timing, not for audio. The whole step is captured as one CUDA graph and replayed, the
@@ -21,6 +22,7 @@ import numpy as np
 import torch
 
 from . import ops
+from .kv4 import KV4Cache
 
 LM, LM_FFN, LOC, LOC_FFN, FSQ = 2048, 6144, 1024, 4096, 512
 NQ, NK, HD = 16, 2, 128
@@ -154,14 +156,19 @@ class Engine:
     LM_TC = ("qkv", "o", "gu", "down", "swiglu")
 
     def __init__(self, B, maxlen=4096, timesteps=10, base_layers=28, res_layers=8, enc_layers=4, dit_layers=4,
-                 cfg=2.0, max_steps=256, min_len=2, seed=0, device="cuda", lm_tc=LM_TC):
+                 cfg=2.0, max_steps=256, min_len=2, seed=0, device="cuda", lm_tc=LM_TC, kv="bf16", kv_pages=None):
+        """kv="int4": the LMs' K and V in 4 bits on pages (KV4Cache, one for both, self.kv4) instead of bf16 slots;
+        kv_pages: pages in all (default: enough for every take at maxlen)."""
         if not 1 <= B <= 1024:
             raise ValueError("takes per GPU must be in 1..1024")
+        if kv not in ("bf16", "int4"):
+            raise ValueError('kv: "bf16" or "int4"')
         self.B, self.maxlen, self.cfg, self.max_steps, self.min_len = B, maxlen, cfg, max_steps, min_len
         self.device = dev = torch.device(device)
         ini = _Init(seed, dev)
-        self.base = Tf(ini, base_layers, LM, LM_FFN, True, B, maxlen, tc=lm_tc)
-        self.res = Tf(ini, res_layers, LM, LM_FFN, False, B, maxlen, tc=lm_tc)  # no rope (src/model.rs:445)
+        slots = B if kv == "bf16" else 0
+        self.base = Tf(ini, base_layers, LM, LM_FFN, True, slots, maxlen, tc=lm_tc)
+        self.res = Tf(ini, res_layers, LM, LM_FFN, False, slots, maxlen, tc=lm_tc)  # no rope (src/model.rs:445)
         self.enc = Tf(ini, enc_layers, LOC, LOC_FFN, True)
         self.dit = Tf(ini, dit_layers, LOC, LOC_FFN, True)
         L = lambda n, k, b=True: Lin(ini, n, k, b)  # noqa: E731
@@ -189,7 +196,11 @@ class Engine:
         self.lens = torch.ones(B, dtype=torch.int32, device=dev)
         self.ctr = torch.zeros(4, dtype=torch.int32, device=dev)
         self.stop = torch.full((B,), -1, dtype=torch.int32, device=dev)
-        self.ws = ops.decode_workspace(B, NQ, NK, HD, maxlen, dev)
+        self.ws = ops.decode_workspace(B, NQ, NK, HD, maxlen, dev) if kv == "bf16" else None
+        self.kv4 = None
+        if kv == "int4":
+            pages = B * -(-maxlen // ops.KV4_PAGE) if kv_pages is None else kv_pages
+            self.kv4 = KV4Cache(base_layers + res_layers, B, NQ, NK, HD, pages, maxlen, dev, lens=self.lens)
         self._scratch = {}
 
     def _temb(self, ini):
@@ -233,22 +244,57 @@ class Engine:
         heads = 2 * B * (2 * LOC * LM + 4 * 64 * LOC + LM * LOC + FSQ * LM * 2 + 2 * LM * LM + LM * LM + 2 * LM)
         return lm + dit + enc + heads
 
-    def prime(self, lens, seed=1):
+    def prime(self, lens, seed=1, prompt=0):
         """Every take holds a prompt: random bf16 K/V in its slots and random hidden states; lens[s] is the number
-        of positions take s attends over in the next step (its newest position, lens[s] - 1, is written by it)."""
+        of positions take s attends over in the next step (its newest position, lens[s] - 1, is written by it). The
+        first `prompt` positions are the same for every take, written once and replicated into the slots, or with the
+        4-bit cache shared (the reference prefills slot 0 and replicates it, src/model.rs:705-717)."""
         lens = [int(v) for v in lens]
-        if len(lens) != self.B or min(lens) < 1 or max(lens) > self.maxlen:
-            raise ValueError("one length in 1..maxlen per take")
+        if len(lens) != self.B or min(lens) < 1 or max(lens) > self.maxlen or not 0 <= prompt < min(lens):
+            raise ValueError("one length in 1..maxlen per take, above the prompt's")
         g = torch.Generator(device=self.device)
         g.manual_seed(seed)
         for tf in (self.base, self.res):
             for c in tf.kc + tf.vc:
                 c.normal_(generator=g)
+                if prompt:
+                    ops.kv_replicate(c, self.B, NK, self.maxlen, HD, prompt)
+        if self.kv4 is not None:
+            self._prime_pages(lens, g, prompt)
         for t in (self.lm_h, self.res_h, self.cond, self.noise):
             t.normal_(generator=g)
         self.set_lens(lens)
 
+    def _prime_pages(self, lens, g, prompt):
+        """Pages with random K/V: the prompt in take 0, forked to the others, then every take's own positions."""
+        c, B, dev = self.kv4, self.B, self.device
+        c.free(range(B))
+        self._prompt = prompt
+        if prompt:
+            row = torch.empty((prompt, 2 * NK * HD), dtype=torch.bfloat16, device=dev)
+            self.lens[0] = prompt
+            c.extend()
+            for l in range(c.layers):
+                ops.kv4_write(row.normal_(generator=g), c.pools[l], c.table, None, None, 1, prompt, 0, NK, HD)
+            if B > 1:
+                c.fork([0] * (B - 1), range(1, B))
+        self.lens.copy_(torch.as_tensor(lens, dtype=torch.int32))
+        c.extend()
+        own = max(lens) - prompt
+        start = torch.full((B,), prompt, dtype=torch.int32, device=dev)
+        rows = torch.empty((B * own, 2 * NK * HD), dtype=torch.bfloat16, device=dev)
+        for l in range(c.layers):
+            c.write(l, rows.normal_(generator=g), own, nq=0, start=start, count=self.lens - prompt)
+        self._check_pages()
+
+    def _check_pages(self):
+        if self.kv4 is not None and int(self.kv4.status[0]):
+            raise RuntimeError(f"the 4-bit cache's {self.kv4.npages} pages do not hold the takes: "
+                               f"{int(self.kv4.status[0])} pages are missing")
+
     def set_lens(self, lens):
+        if self.kv4 is not None and min(int(v) for v in lens) <= getattr(self, "_prompt", 0):
+            raise ValueError("a take's newest position lies behind the prompt it shares")
         self.lens.copy_(torch.as_tensor([int(v) for v in lens], dtype=torch.int32))
         self.ctr.zero_()
         self.stop.fill_(-1)
@@ -296,6 +342,11 @@ class Engine:
         ops.rmsnorm(x, tf.layers[0]["ln1"], sc["xn"], EPS)
         for li, l in enumerate(tf.layers):
             l["qkv"](sc["xn"], sc["qkv"])
+            if self.kv4 is not None:
+                self.kv4.step(li + (0 if tf is self.base else len(self.base.layers)), sc["qkv"], sc["att"],
+                              self.cos if tf.rope else None, self.sin if tf.rope else None)
+                self._post_attn(tf, li, x, sc, out)
+                continue
             ops.step_tf_attention(sc["qkv"], tf.kc[li], tf.vc[li], sc["att"], self.ws, self.cos, self.sin, None,
                                   self.lens, B, NQ, NK, HD, self.maxlen, rope_on=tf.rope)
             self._post_attn(tf, li, x, sc, out)
@@ -313,6 +364,8 @@ class Engine:
     def step(self):
         """One decoding step for every take; device work only, so it can be captured (src/model.rs:725-773)."""
         B = self.B
+        if self.kv4 is not None:
+            self.kv4.extend()  # lens counts the position this step writes
         self.lm_to_dit(self.lm_h, self.mu[:, :LOC])
         self.res_to_dit(self.res_h, self.mu[:, LOC:])
         self.dit_cond(self.cond.view(B * 4, 64), self.condp)
@@ -384,4 +437,5 @@ class Engine:
                     break
                 graph.replay()
                 stops = self.stop.cpu()
+        self._check_pages()
         return [int(v) + 1 if v >= 0 else self.max_steps for v in stops.tolist()]

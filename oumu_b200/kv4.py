@@ -1,0 +1,67 @@
+"""The 4-bit paged KV cache of a set of layers: the buffers oumu_kv4_*, oumu_attn_decode_kv4* and oumu_pages_* work on
+(include/oumu_attn.h) and the calls on them. Takes the place of the bf16 slots [slots][nk][maxlen][hd] of the reference
+engine (src/model.rs:130-133) in 0.31 of their bytes, with memory for the positions takes hold instead of the longest
+take's for every one, and the prompt held once for all takes that start from it (src/model.rs:705-717 copies it into
+every slot)."""
+import torch
+
+from . import ops
+
+
+class KV4Cache:
+    """`layers` layers of `npages` pages for B takes of up to maxlen positions. `lens` (int32 [B], device) holds the takes'
+    lengths; a caller that advances its own on the device (oumu_step_end) passes it. Everything is enqueued on the
+    current stream and can be captured; nothing here waits for the GPU."""
+
+    def __init__(self, layers, B, nq, nk, hd, npages, maxlen, device="cuda", lens=None):
+        self.layers, self.B, self.nq, self.nk, self.hd, self.npages = layers, B, nq, nk, hd, npages
+        self.maxpages = -(-maxlen // ops.KV4_PAGE)
+        if layers < 1 or B < 1 or npages < 1 or maxlen < 1:
+            raise ValueError("a cache has layers, takes, pages and positions")
+        dev = torch.device(device)
+        i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)  # noqa: E731
+        self.pools = torch.empty((layers, npages, ops.kv4_page_bytes(nk, hd)), dtype=torch.uint8, device=dev)
+        self.table = torch.full((B, self.maxpages), -1, dtype=torch.int32, device=dev)
+        self.ref, self.lens = i32(npages), i32(B) if lens is None else lens
+        self.status, self.moved = i32(2), i32(2)  # [pages missing], [pages in use, pages moved]
+        self.ws = ops.decode_kv4_workspace(B, nq, nk, hd, self.maxpages, dev)
+        self._pages_ws = ops.pages_workspace(npages, dev)
+
+    def _ids(self, takes):
+        return torch.as_tensor(takes, dtype=torch.int32).to(self.table.device)
+
+    def extend(self, extra=0):
+        """Pages for every take's first lens + extra positions; status[0] counts those the pool did not have."""
+        ops.pages_extend(self.table, self.ref, self.lens, extra, self.status)
+
+    def fork(self, src, dst):
+        """Takes dst[i] continue where takes src[i] are, on shared pages (device int32 tensors, or lists)."""
+        ops.pages_fork(self.pools, self.table, self.ref, self.lens, self._ids(src), self._ids(dst), self.status)
+
+    def free(self, takes):
+        ops.pages_free(self.table, self.ref, self.lens, self._ids(takes))
+
+    def compact(self):
+        """Pages in use to the front of the pools; moved = [pages in use, pages moved]."""
+        ops.pages_compact(self.pools, self.table, self.ref, self._pages_ws, self.moved)
+
+    def write(self, layer, qkv, rows, nq=None, start=None, count=None):
+        """k and v of `rows` rows per take of qkv (nq q heads before them, by default the cache's) at start[s] + i."""
+        ops.kv4_write(qkv, self.pools[layer], self.table, start, count, self.B, rows, self.nq if nq is None else nq,
+                      self.nk, self.hd)
+
+    def read(self, layer, kc, vc):
+        """What the takes hold, as bf16 slots [B][nk][maxlen][hd]."""
+        ops.kv4_read(self.pools[layer], self.table, self.lens, kc, vc, self.nk, self.hd)
+
+    def attend(self, layer, qkv, out, scale=None):
+        ops.attn_decode_kv4(qkv, self.pools[layer], out, self.ws, self.table, None, self.lens, self.B, self.nq, self.nk,
+                            self.hd, self.hd ** -0.5 if scale is None else scale)
+
+    def step(self, layer, qkv, out, cos_t=None, sin_t=None, scale=None, held=None):
+        """One decode layer: rope, quantisation, cache write and attention of every take's newest position."""
+        ops.attn_decode_kv4_step(qkv, self.pools[layer], out, self.ws, cos_t, sin_t, self.table, None, self.lens, self.B,
+                                 self.nq, self.nk, self.hd, self.hd ** -0.5 if scale is None else scale, held=held)
+
+    def nbytes(self):
+        return self.pools.numel()

@@ -21,6 +21,13 @@ def _stream():
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
+def _ints(dev, *ts):
+    """Tables, counts, lengths and takes of the paged cache."""
+    for t in ts:
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev):
+            raise ValueError("page tables, counts, lengths and takes: contiguous int32 tensors on the current device")
+
+
 def rotary_tables(maxlen, hd, ext=None):
     """cos, sin fp32 [maxlen][hd/2] built on the host (src/model.rs:337-349), as CPU tensors."""
     import ctypes
@@ -297,9 +304,7 @@ def _kv4_check(pool, table, *ints, nk=0, hd=0, B=0):
     dev = torch.cuda.current_device()
     if pool.get_device() != dev:
         raise ValueError("the cache is not on the current device")
-    for t in (table, *ints):
-        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev):
-            raise ValueError("page tables, counts, lengths and takes: contiguous int32 tensors on the current device")
+    _ints(dev, table, *ints)
 
 
 def _takes(n, *ts):
@@ -362,8 +367,15 @@ def attn_decode_kv4_step(qkv, pool, out, workspace, cos_t, sin_t, table, pos, le
     _rows(qkv, B * (nq + 2 * nk) * hd, "qkv")
     _rows(out, B * nq * hd, "out")
     _rows(held, B * 2 * nk * hd, "held")
+    rows = 0
+    if cos_t is not None:
+        rows = cos_t.shape[0]
+        if (sin_t is None or cos_t.dtype is not torch.float32 or sin_t.dtype is not torch.float32
+                or cos_t.shape != (rows, hd // 2) or sin_t.shape != cos_t.shape
+                or not cos_t.is_contiguous() or not sin_t.is_contiguous()):
+            raise ValueError("cos_t and sin_t: contiguous fp32 [rows][hd / 2]")
     _lib.call("oumu_attn_decode_kv4_step", _p(qkv), _p(pool), _p(out), _p(held), _p(workspace), workspace.numel(),
-              _p(cos_t), _p(sin_t), _p(table), _p(pos), _p(lens), B, nq, nk, hd, pool.shape[0], table.shape[1],
+              _p(cos_t), _p(sin_t), rows, _p(table), _p(pos), _p(lens), B, nq, nk, hd, pool.shape[0], table.shape[1],
               float(scale), _stream())
 
 
@@ -376,10 +388,7 @@ def _pools(pools, ref):
 def pages_extend(table, ref, lens, extra, status):
     """Every take that holds positions gets the pages it lacks for lens[s] + extra of them (oumu_pages_extend);
     status[0]: pages missing."""
-    dev = torch.cuda.current_device()
-    for t in (table, ref, lens, status):
-        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev:
-            raise ValueError("page tables, counts, lengths and takes: contiguous int32 tensors on the current device")
+    _ints(torch.cuda.current_device(), table, ref, lens, status)
     if table.dim() != 2 or lens.numel() < table.shape[0] or status.numel() < 1:
         raise ValueError("table: [B][maxpages], lens: [B], status: [1]")
     _lib.call("oumu_pages_extend", _p(table), _p(ref), _p(lens), extra, _p(status), table.shape[0], ref.numel(),
@@ -398,10 +407,7 @@ def pages_fork(pools, table, ref, lens, src, dst, status):
 
 def pages_free(table, ref, lens, takes):
     """The takes give their pages back and are empty (oumu_pages_free)."""
-    dev = torch.cuda.current_device()
-    for t in (table, ref, lens, takes):
-        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev:
-            raise ValueError("page tables, counts, lengths and takes: contiguous int32 tensors on the current device")
+    _ints(torch.cuda.current_device(), table, ref, lens, takes)
     if table.dim() != 2 or lens.numel() < table.shape[0]:
         raise ValueError("table: [B][maxpages], lens: [B]")
     _lib.call("oumu_pages_free", _p(table), _p(ref), _p(lens), _p(takes), takes.numel(), table.shape[0], ref.numel(),

@@ -70,8 +70,9 @@ def test_attention_refusals(lib):
     assert attn(B=4096, maxpages=1 << 18) == UNSUPPORTED  # more tiles than the kernel counts
     assert attn(n=256) == WORKSPACE
     step = lib.oumu_attn_decode_kv4_step
-    assert step(P, P, P, ODD, P, 1 << 24, P, P, P, None, P, 4, 16, 2, 128, 8, 8, 0.1, None) == INVALID
-    assert step(P, P, P, None, P, 1 << 24, P, None, P, None, P, 4, 16, 2, 128, 8, 8, 0.1, None) == INVALID
+    assert step(P, P, P, ODD, P, 1 << 24, P, P, 512, P, None, P, 4, 16, 2, 128, 8, 8, 0.1, None) == INVALID
+    assert step(P, P, P, None, P, 1 << 24, P, None, 512, P, None, P, 4, 16, 2, 128, 8, 8, 0.1, None) == INVALID
+    assert step(P, P, P, None, P, 1 << 24, P, P, 0, P, None, P, 4, 16, 2, 128, 8, 8, 0.1, None) == INVALID
     assert lib.oumu_attn_decode_kv4_workspace(4, 18, 2, 128, 8) == 0
     assert lib.oumu_attn_decode_kv4_workspace(4, 16, 2, 128, 0) == 0
     assert lib.oumu_attn_decode_kv4_workspace(4, 16, 2, 128, 8) > 0
