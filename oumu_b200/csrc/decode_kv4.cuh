@@ -544,9 +544,9 @@ constexpr int MIN_TILES = NW;
 template <int NW>
 constexpr int SNAP = 3 * NW;
 
-// A segment that crosses a boundary: take * nk + kv head, its tiles, the CTA's warps that have some of them.
-struct Cross {
-    int id, start, end, first, last;
+// A segment that a boundary cuts: take * nk + kv head (-1: none), its tiles.
+struct Cut {
+    int id, start, end;
 };
 
 template <int HD, int NW>
@@ -558,8 +558,8 @@ struct Lay {
     static_assert(REC * 4 <= RING, "a warp's last record lies in its own ring");
     static constexpr int FIRST = NW * RING;           // records of segments that end inside a warp's range
     static constexpr int BAR = FIRST + NW * REC * 4;
-    static constexpr int LIST = BAR + NW * ST<NW> * 8;    // segments that cross warps
-    static constexpr int MISC = LIST + (NW + 1) * static_cast<int>(sizeof(Cross));
+    static constexpr int CUTS = BAR + NW * ST<NW> * 8;    // segments cut by the warps' boundaries
+    static constexpr int MISC = CUTS + (NW + 1) * static_cast<int>(sizeof(Cut));
     static constexpr int PRE = MISC + 128;            // pre[B + 1], lens[B]
     static __host__ __device__ int bytes(int B) { return PRE + (2 * B + 1) * 4; }
 };
@@ -686,39 +686,20 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
     const Parts parts(tb - ta, NW);
     const int wa = ta + parts.start(warp), wb = ta + parts.start(warp + 1), n = wb - wa;
 
-    Cross *list = reinterpret_cast<Cross *>(sm + Y::LIST);
-    auto list_crossings = [&] {
-        // Boundary b (where warp b starts; b == NW: the CTA's end) lies inside a segment, which may be the one before it
-        // again, or between two.
-        Cross x{-1, 0, 0, 0, 0};
-        const int at = ta + parts.start(lane < NW ? lane : NW);
-        const bool any = lane < NW ? at < tb : lane == NW;  // a warp without tiles starts where the CTA ends
-        if (any) {
-            // the segment of tile `at`, at the CTA's end of the tile before: its start is known to the warp that has it
-            const int s = take_of(pre, B, lane < NW ? at : tb - 1), T = tiles_of<HD>(Ls[s]);
-            const int kh = ((lane < NW ? at : tb - 1) - pre[s]) / T;
-            x.id = s * nk + kh;
-            x.start = pre[s] + kh * T;
-            x.end = x.start + T;
-            if (x.start >= at || x.end <= at) x.id = -1;  // starts here, or ends here
-        }
-        // the boundary before it, that of the last warp with tiles for the CTA's end
-        const int before = __shfl_sync(0xffffffffu, x.id, lane == NW ? min(NW, tb - ta) - 1 : lane - 1);
-        const unsigned in = __ballot_sync(0xffffffffu, x.id >= 0 && (lane == 0 || x.id != before));
-        if (in >> lane & 1) {
-            x.first = parts.of(max(x.start, ta) - ta);
-            x.last = parts.of(min(x.end, tb) - 1 - ta);
-            list[__popc(in & ((1u << lane) - 1))] = x;
-        }
-        if (lane == 0) misc[0] = __popc(in);
-    };
+    // Boundary b of the CTA's range (b < nb: where warp b starts; nb, the number of warps with tiles: the range's end) and
+    // the segment it cuts, each found by the warp that has it at hand; id -1 where a segment ends there.
+    Cut *cuts = reinterpret_cast<Cut *>(sm + Y::CUTS);
+    const int nb = min(NW, tb - ta);
     // ---- this warp's tiles ----
     if (n > 0) {
         const uint8_t *src = nullptr;  // lane i: tile base + i
+        int s, T, kh, j;               // its take, tiles of a segment, kv head, tile of the segment
         auto look_up = [&](int base) {
-            const int t = wa + base + lane;
-            if (t >= wb) return;
-            const int s = take_of(pre, B, t), T = tiles_of<HD>(Ls[s]), off = t - pre[s], kh = off / T, j = off - kh * T;
+            const int t = min(wa + base + lane, wb - 1);
+            s = take_of(pre, B, t);
+            T = tiles_of<HD>(Ls[s]);
+            kh = (t - pre[s]) / T;
+            j = t - pre[s] - kh * T;
             constexpr int per = kv4::PAGE / TP;  // tiles of a page
             int page = P.table[static_cast<long>(s) * P.maxpages + j / per];
             if (page < 0 || page >= P.npages) {
@@ -734,11 +715,19 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         // Fused, a copy may come before the preceding kernel's end: that kernel writes no page, and the newest position is
         // patched in. Otherwise it may be the write of the newest position.
         if (!FUSED) after_predecessor();
+        auto look_up_later = [&](int base) {  // with s .. j kept: they are the warp's place by then
+            const int s0 = s, T0 = T, kh0 = kh, j0 = j;
+            look_up(base);
+            s = s0, T = T0, kh = kh0, j = j0;
+        };
         look_up(0);
         issue(0);
-        if (warp == 0) list_crossings();  // while the first copies are on their way
         if (FUSED) after_predecessor();
-        int s = take_of(pre, B, wa), T = tiles_of<HD>(Ls[s]), kh = (wa - pre[s]) / T, j = wa - pre[s] - kh * T;
+        s = __shfl_sync(0xffffffffu, s, 0);
+        T = __shfl_sync(0xffffffffu, T, 0);
+        kh = __shfl_sync(0xffffffffu, kh, 0);
+        j = __shfl_sync(0xffffffffu, j, 0);
+        if (lane == 0) cuts[warp] = Cut{j > 0 ? s * nk + kh : -1, wa - j, wa - j + T};
         int k = 0, issued = 1;
         while (k < n) {
             // ---- this warp's part of a segment: tiles j .. of take s, kv head kh ----
@@ -772,7 +761,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
                 for (int h = 0; h < TP / HALF && left > h * HALF; h++) S.tile(half + h * F::HALFB, left - h * HALF, Q, lane);
                 __syncwarp();
                 if (issued < n) {
-                    if ((issued & 31) == 0) look_up(issued);
+                    if ((issued & 31) == 0) look_up_later(issued);
                     issue(issued++);
                 }
             }
@@ -780,6 +769,11 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
                 // A wait ran out (recorded): nothing more is computed or started; the outputs are unspecified, but no
                 // copy may still be on its way when the CTA leaves (bounded again).
                 for (int i = k; i < issued; i++) mbar_wait(bars + 8 * (i % ST), (i / ST) & 1);
+                if (warp == nb - 1 && lane == 0) {  // what this warp would have found at its end
+                    const int s1 = take_of(pre, B, tb - 1), T1 = tiles_of<HD>(Ls[s1]), h1 = (tb - 1 - pre[s1]) / T1;
+                    const int g1 = pre[s1] + h1 * T1;
+                    cuts[nb] = Cut{g1 + T1 > tb ? s1 * nk + h1 : -1, g1, g1 + T1};
+                }
                 break;
             }
             if (ends && Sg >= wa) {
@@ -789,6 +783,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
                                 : reinterpret_cast<float *>(sm + Y::FIRST) + warp * Y::REC,
                          lane);
             }
+            if (k == n && warp == nb - 1 && lane == 0) cuts[nb] = Cut{ends ? -1 : s * nk + kh, Sg, Sg + T};
             j = 0;
             if (++kh == nk) {
                 kh = 0;
@@ -803,7 +798,6 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
 
     // ---- segments that cross a boundary between warps, or the CTA's ends ----
     // The loops here are not unrolled: run once per launch, they cost their instruction fetches.
-    const int nlist = misc[0];
     constexpr int LPH = HD / 4;  // threads per head, 4 channels each
     const int h = threadIdx.x / LPH, d4 = threadIdx.x % LPH;
     auto store = [&](int id, float l, float4 o) {
@@ -817,12 +811,20 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         l = fmaf(f, lw, l);
         o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
     };
-    int crossing = 0;  // entries that reach into other CTAs: the first, the last, or none
+    int crossing = 0;  // bit 0: the segment cut by the range's start, bit 1: by its end only, reaches into other CTAs
+    // boundaries that cut a segment for the first time, and those that cut the one before's again (a lane per boundary)
+    const int mine = lane <= nb ? cuts[lane].id : -1, left_one = __shfl_up_sync(0xffffffffu, mine, 1);
+    const bool again = lane > 0 && mine == left_one;
+    unsigned todo = __ballot_sync(0xffffffffu, mine >= 0 && !again);
+    const unsigned more = __ballot_sync(0xffffffffu, mine >= 0 && again);
 #pragma unroll 1
-    for (int i = 0; i < nlist; i++) {
-        const Cross x = list[i];
+    for (; todo; todo &= todo - 1) {
+        const int i = __ffs(todo) - 1;
+        const Cut x = cuts[i];
+        // the warps that have some of it: from the one before its first boundary to the one behind its last
+        const int first = max(i - 1, 0), last = min(i + __ffs(~(more >> i >> 1)) - 1, nb - 1);
         const bool out = x.start < ta || x.end > tb;
-        crossing |= out << (i > 0 && i == nlist - 1);
+        if (out) crossing |= x.start < ta ? 1 : 2;
         if (h >= G) continue;
         auto at = [&](int w) {  // warp w's record of it: its last one if the segment goes on to the range's end
             return x.end >= ta + parts.start(w + 1) ? reinterpret_cast<const float *>(sm + w * Y::RING)
@@ -830,21 +832,21 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         };
         // the head's LPH threads take a record's reference and sum each
         const unsigned mates = LPH == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
-        const bool has = x.first + d4 <= x.last;
-        const float m = has ? at(x.first + d4)[h] : -INFINITY;
+        const bool has = first + d4 <= last;
+        const float m = has ? at(first + d4)[h] : -INFINITY;
         float M = m;
 #pragma unroll
         for (int e = 1; e < 16; e <<= 1) M = fmaxf(M, __shfl_xor_sync(mates, M, e, 16));
         M = __shfl_sync(mates, M, 0, LPH);
         const float fm = fast_exp2(m - M);
-        float l = has ? fm * at(x.first + d4)[GMAX + h] : 0.f;
+        float l = has ? fm * at(first + d4)[GMAX + h] : 0.f;
 #pragma unroll
         for (int e = 1; e < 16; e <<= 1) l += __shfl_xor_sync(mates, l, e, 16);
         l = __shfl_sync(mates, l, 0, LPH);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
-        for (int w = x.first; w <= x.last; w++) {
-            const float f = __shfl_sync(mates, fm, w - x.first, LPH);
+        for (int w = first; w <= last; w++) {
+            const float f = __shfl_sync(mates, fm, w - first, LPH);
             const float4 v = *reinterpret_cast<const float4 *>(at(w) + 2 * GMAX + h * HD + 4 * d4);
             o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
         }
@@ -863,7 +865,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
     // the counts of the (at most two) segments that reach into other CTAs; whoever completes one adds it up
     __syncthreads();
     if (threadIdx.x < 2 && crossing >> threadIdx.x & 1) {
-        const Cross x = list[threadIdx.x ? nlist - 1 : 0];
+        const Cut x = cuts[threadIdx.x ? nb : 0];
         const int others = ctas.of(x.end - 1) - ctas.of(x.start);
         const bool done = atomic_add_acq_rel(P.cnt + x.id, 1) == others;
         if (done) P.cnt[x.id] = 0;
@@ -873,7 +875,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
 #pragma unroll 1
     for (int k = 0; k < 2; k++) {
         if (!(crossing >> k & 1) || !misc[1 + k] || h >= G) continue;
-        const Cross x = list[k ? nlist - 1 : 0];
+        const Cut x = cuts[k ? nb : 0];
         const int cf = ctas.of(x.start), cl = ctas.of(x.end - 1);
         auto at = [&](int cc) { return P.part + (static_cast<long>(cc) * 2 + (cc == cf)) * Y::REC + h; };
         auto numer = [&](int cc) {
