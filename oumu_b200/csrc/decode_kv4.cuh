@@ -502,7 +502,12 @@ struct Newest {
             for (int o = 1; o < 8; o <<= 1) rg = kv4::range_max(rg, __shfl_xor_sync(0xffffffffu, rg, o));
             const kv4::Quant q = kv4::quant_of(rg);
             const uint32_t pr[2] = {u[kv].x, u[kv].y};
-            const uint32_t c = kv4::quant_pairs<2>(pr, q);  // low half: channels 0, 2; high half: 1, 3
+            uint32_t marks = 0, c = kv4::quant_pairs<2>(pr, q, marks);  // low half: channels 0, 2; high half: 1, 3
+            if (marks & 1u && kv4::quant_marked<2>(pr, q.s, q.z, c)) {
+                const float2 f0 = unpack_bf16x2(pr[0]), f1 = unpack_bf16x2(pr[1]);
+                c = kv4::quant_exact(f0.x, q.z, q.s) | kv4::quant_exact(f0.y, q.z, q.s) << 16 |
+                    kv4::quant_exact(f1.x, q.z, q.s) << 4 | kv4::quant_exact(f1.y, q.z, q.s) << 20;
+            }
             const uint32_t n[4] = {c & 15u, c >> 16 & 15u, c >> 4 & 15u, c >> 20 & 15u};
             if (P.held && on) {
                 uint2 o;
@@ -514,7 +519,7 @@ struct Newest {
                 const uint32_t kw = (c & 0x00ff00ffu) << (8 * (j & 1));
                 code[0] = kw | __shfl_xor_sync(0xffffffffu, kw, 1);
             } else {
-                code[1] = n[0] | n[1] << 4 | n[2] << 8 | n[3] << 12;
+                code[1] = kv4::in_order(c);
             }
             meta[kv] = kv4::meta_bits(q.s, q.z);
         }

@@ -81,8 +81,9 @@ __device__ __forceinline__ uint32_t range_of(uint32_t mx2, uint32_t mn2) {  // p
 __device__ __forceinline__ uint32_t range_max(uint32_t a, uint32_t b) { return as_u32(__hmax2_nan(as_bf2(a), as_bf2(b))); }
 
 struct Quant {
-    float s, z, rinv;
+    float s, z, rinv;  // rinv: 1 / s, its last bit a mark (see quant_of); 0 for a scale of 0 or NaN
 };
+constexpr float TINY = 0.000244140625f;  // 2^-12
 // s, the smallest bf16 >= D / 15 with D = max - min rounded up in fp32 (15 s has 12 bits, so rounding D up to fp32 does
 // not change which s is enough): D times a float a little above 1 / 15, cut to bf16, is it or the one before it, and
 // 15 s >= D, exact, tells. A scale that is not finite becomes NaN.
@@ -95,68 +96,84 @@ __device__ __forceinline__ Quant quant_of(uint32_t range) {
     q.s = __uint_as_float(15.f * __uint_as_float(b) >= D ? b : b + 0x10000u);
     if (!(D < 3.4e38f)) q.s = __uint_as_float(0x7fc00000u);
     q.rinv = __fdividef(1.f, q.s);
+    // quant_pairs takes x - z as fp32 has it, which is exact for ordinary groups: where z is 0 or at least 2^-12 s, and x
+    // too, both are multiples of 2^-19 of the power of two at or below s, and the difference is below 2^5 of it. Where x
+    // is smaller, but not 0, x - z is far from every border unless 0 itself lies on one. The last bit of 1 / s marks
+    // groups that may be other than that, and scales without a normal reciprocal.
+    const float n = __fadd_rn(fmaf(-q.z, q.rinv, 12582912.f), -12582912.f);
+    const bool odd = fabsf(fmaf(-n, q.s, -q.z)) == 0.5f * q.s || (q.z != 0.f && fabsf(q.z) < q.s * TINY) || q.s < 7.9e-31f;
+    q.rinv = q.s > 0.f ? __uint_as_float((__float_as_uint(q.rinv) & ~1u) | odd) : 0.f;
     return q;
 }
-// The nearest multiple decided exactly, for a group of which some value lies on a border (among bf16 numbers ties are
-// common) or whose scale has no normal reciprocal: x - z = d + e (two-sum), r = d - n s exactly (n s has 12 bits, n is
-// at most one off).
-__device__ __forceinline__ uint32_t quant_exact(float x, const Quant &q) {
-    const float d = __fsub_rn(x, q.z);
-    const float bb = __fsub_rn(d, x);
-    const float e = __fadd_rn(__fsub_rn(x, __fsub_rn(d, bb)), __fsub_rn(-q.z, bb));
-    float n = fminf(fmaxf(rintf(q.rinv < 1.7e38f ? d * q.rinv : __fdiv_rn(d, q.s)), 0.f), 15.f);
-    const float r = fmaf(-n, q.s, d), h = 0.5f * q.s;
+// The nearest multiple decided exactly: x - z = d + e (two-sum), r = d - n s (n s has 12 bits, n is at most one off), all
+// times a power of two where 1 / s would not be a normal number.
+__device__ __forceinline__ uint32_t quant_exact(float x, float z, float s) {
+    if (!(s > 0.f)) return 0u;
+    const float up = s < 9.1e-13f ? 1.2676506e30f : 1.f;  // 2^100 for scales below 2^-40
+    const float dx = __fsub_rn(x, z), bb = __fsub_rn(dx, x);
+    const float e = __fadd_rn(__fsub_rn(x, __fsub_rn(dx, bb)), __fsub_rn(-z, bb));
+    const float d = dx * up, sc = s * up, h = 0.5f * sc;
+    float n = fminf(fmaxf(rintf(d * __fdividef(1.f, sc)), 0.f), 15.f);
+    const float r = fmaf(-n, sc, d);
     const bool odd = static_cast<int>(n) & 1;
     if (r > h || (r == h && (e > 0.f || (e == 0.f && odd)))) n += 1.f;
     else if (r < -h || (r == -h && (e < 0.f || (e == 0.f && odd)))) n -= 1.f;
-    return q.s > 0.f ? static_cast<uint32_t>(n) : 0u;
-}
-template <int NP>
-__device__ __noinline__ uint32_t quant_pairs_exact(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, Quant q) {
-    const uint32_t x[4] = {x0, x1, x2, x3};
-    uint32_t lo = 0, hi = 0;
-#pragma unroll
-    for (int i = NP - 1; i >= 0; i--) {
-        const float2 f = unpack_bf16x2(x[i]);
-        lo = lo * 16u + quant_exact(f.x, q);
-        hi = hi * 16u + quant_exact(f.y, q);
-    }
-    return lo | hi << 16;
+    return static_cast<uint32_t>(n);
 }
 // The codes of NP bf16 pairs, nibble i of the low and high half being pair i's two values. The quotient (x - z) / s is
-// corrected to the nearest float, so a tie among whole numbers is one exactly and adding 1.5 * 2^23 rounds it to even (n
-// is then in the low bits). Each n is right where the remainder is below s / 2, or s / 2 itself and x - z exact.
+// corrected to the nearest float, so a tie among whole numbers is one exactly (among bf16 numbers ties are common: one
+// value in 370 of normal ones) and nothing else becomes one, being 2^-20 or more off; adding 1.5 * 2^23 rounds it, ties to
+// even, and leaves n in the low bits. `marks` collects 1 / s: where its last bit is set, quant_marked has to look at these
+// codes. (Checks behind each group would cost as much as the codes.)
 template <int NP>
-__device__ __forceinline__ uint32_t quant_pairs(const uint32_t (&x)[NP], const Quant &q) {
-    const float magic = 12582912.f, h = 0.5f * q.s;
+__device__ __forceinline__ uint32_t quant_pairs(const uint32_t (&x)[NP], const Quant &q, uint32_t &marks) {
+    const float magic = 12582912.f;
     const float2 rv = make_float2(q.rinv, q.rinv), ms = make_float2(-q.s, -q.s);
-    const float2 mz = make_float2(-q.z, -q.z), mg = make_float2(magic, magic), back = make_float2(-magic, -magic);
+    const float2 mz = make_float2(-q.z, -q.z), mg = make_float2(magic, magic);
     uint32_t lo = 0, hi = 0;
-    float far = q.rinv < 1.7e38f ? 0.f : INFINITY;  // no normal reciprocal: a scale of 0 or below 2^-127
-    float2 f[NP], d[NP], r[NP];
 #pragma unroll
     for (int i = NP - 1; i >= 0; i--) {
-        f[i] = make_float2(__uint_as_float(x[i] << 16), __uint_as_float(x[i] & 0xffff0000u));
-        d[i] = add2(f[i], mz);
-        const float2 t = mul2(d[i], rv);
-        const float2 a = add2(fma2(fma2(t, ms, d[i]), rv, t), mg);
-        r[i] = fma2(add2(a, back), ms, d[i]);
-        far = fmax3(far, fabsf(r[i].x), fabsf(r[i].y));
+        const float2 d = add2(make_float2(__uint_as_float(x[i] << 16), __uint_as_float(x[i] & 0xffff0000u)), mz);
+        const float2 t = mul2(d, rv);
+        const float2 a = add2(fma2(fma2(t, ms, d), rv, t), mg);
         lo = lo * 16u + __float_as_uint(a.x);  // the magic number's own bits leave the low 16
         hi = hi * 16u + __float_as_uint(a.y);
     }
-    if (!(far < h)) {
-        // a tie (among bf16 numbers common), or something rarer
-        bool odd = !(far <= h);
-#pragma unroll
-        for (int i = 0; i < NP; i++)
-            odd = odd || __fadd_rn(d[i].x, q.z) != f[i].x || __fadd_rn(d[i].y, q.z) != f[i].y;
-        if (odd) return quant_pairs_exact<NP>(x[0], x[1], x[NP - 2], x[NP - 1], q);
-    }
+    marks |= __float_as_uint(q.rinv);
     return __byte_perm(lo, hi, 0x5410);
+}
+// What a mark stands for, in the codes of quant_pairs: where 0 lies on a border, -z = (m + 1/2) s, a value tiny beside s
+// has m + 1 or m by its sign. True where the codes have to be made by quant_exact instead.
+template <int NP>
+__device__ __forceinline__ bool quant_marked(const uint32_t (&x)[NP], float s, float z, uint32_t &code) {
+    const float n = rintf(-z * __fdividef(1.f, s)), r = fmaf(-n, s, -z), tiny = s * TINY;
+    if (fabsf(r) == 0.5f * s) {
+        const uint32_t m = static_cast<uint32_t>(r > 0.f ? n : n - 1.f);
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const float2 f = unpack_bf16x2(x[i]);
+            if (f.x != 0.f && fabsf(f.x) < tiny) code = (code & ~(15u << (4 * i))) | (m + (f.x > 0.f)) << (4 * i);
+            if (f.y != 0.f && fabsf(f.y) < tiny)
+                code = (code & ~(15u << (4 * i + 16))) | (m + (f.y > 0.f)) << (4 * i + 16);
+        }
+    }
+    return (z != 0.f && fabsf(z) < tiny) || (s > 0.f && s < 7.9e-31f);
+}
+// Four nibbles of two pairs' codes (the low half's two, the high half's two) in the order of the four values
+__device__ __forceinline__ uint32_t in_order(uint32_t c) {
+    return (c & 0xfu) | (c >> 12 & 0xf0u) | (c << 4 & 0xf00u) | (c >> 8 & 0xf000u);
 }
 __device__ __forceinline__ uint32_t meta_bits(float a, float b) {  // two bf16-valued floats as a bf16 pair
     return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+}
+__device__ __forceinline__ float scale_of(uint32_t meta) { return __uint_as_float(meta << 16); }
+__device__ __forceinline__ float zero_of(uint32_t meta) { return __uint_as_float(meta & 0xffff0000u); }
+__device__ __forceinline__ Quant quant_from(uint32_t meta, float rinv) {  // of meta_bits(s, z)
+    Quant q;
+    q.s = __uint_as_float(meta << 16);
+    q.z = __uint_as_float(meta & 0xffff0000u);
+    q.rinv = rinv;
+    return q;
 }
 
 // The page of position p of take s: its unit of kv head h, or null (recorded) where the table names no page.
@@ -187,15 +204,185 @@ struct Part {
     }
 };
 
+// A part's rows, where they go, and the work on one of its blocks: true where the codes have to be made again.
+template <int HD>
+struct WriteTo {
+    using F = Fmt<HD>;
+    static constexpr int W = F::W;
+    const bf16 *src;  // row of position p of this head's k or v: src + p * pitch
+    long pitch;
+    uint8_t *u;       // the page's unit
+    int p0, n, lane;  // rows of positions p0 .. p0 + n - 1
+    __device__ __forceinline__ bool ok(int p) const { return p >= p0 && p < p0 + n; }
+
+    __device__ __forceinline__ void load(int b, uint4 (&x)[W]) const {
+        const int p = b * 8 + (lane >> 2);
+#pragma unroll
+        for (int w = 0; w < W; w++)
+            x[w] = ok(p) ? __ldcs(reinterpret_cast<const uint4 *>(src + p * pitch + 32 * w + 8 * (lane & 3)))
+                         : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(int b, uint2 (&x)[2][W]) const {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int p = b * 8 + 2 * (lane & 3) + e;
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                x[e][w] = ok(p) ? __ldcs(reinterpret_cast<const uint2 *>(src + p * pitch + 32 * w + 4 * (lane >> 2)))
+                                : make_uint2(0, 0);
+        }
+    }
+
+    // K: lane 4g + t has channels 32w + 8t .. + 7 of position g
+    __device__ __forceinline__ bool k_block(int b, const uint4 (&x)[W]) const {
+        const int g = lane >> 2, t = lane & 3;
+        Words<W> code, meta;
+        uint32_t sz[W], marks = 0;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const uint32_t xu[4] = {x[w].x, x[w].y, x[w].z, x[w].w};
+            uint32_t mx = xu[0], mn = xu[0];
+#pragma unroll
+            for (int i = 1; i < 4; i++) {
+                mx = as_u32(__hmax2_nan(as_bf2(mx), as_bf2(xu[i])));
+                mn = as_u32(__hmin2_nan(as_bf2(mn), as_bf2(xu[i])));
+            }
+            uint32_t rg = range_of(mx, mn);
+            rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, 1));
+            rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, 2));
+            const Quant q = quant_of(rg);
+            code.v[w] = quant_pairs<4>(xu, q, marks);
+            sz[w] = meta_bits(q.s, q.z);
+        }
+        if (!ok(b * 8 + g)) return false;
+        bool open = false;
+        if (marks & 1u) {
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const uint32_t xu[4] = {x[w].x, x[w].y, x[w].z, x[w].w};
+                open = quant_marked<4>(xu, scale_of(sz[w]), zero_of(sz[w]), code.v[w]) || open;
+            }
+        }
+        uint8_t *half = u + (b & 7) / 4 * F::HALFB;
+        st_words<W>(half + (b & 3) * F::BLOCK + lane * 4 * W, code);
+        if (t == 0) {
+#pragma unroll
+            for (int w = 0; w < W; w += 2) {
+                meta.v[w / 2] = __byte_perm(sz[w], sz[w + 1], 0x5410);
+                meta.v[W / 2 + w / 2] = __byte_perm(sz[w], sz[w + 1], 0x7632);
+            }
+            st_words<W>(half + F::KMETA + ((b & 3) * 8 + g) * F::ROW, meta);
+        }
+        return open;
+    }
+
+    // V: lane 4g + t has channels 32w + 4g .. + 3 of positions 2t and 2t + 1
+    __device__ __forceinline__ bool v_block(int b, const uint2 (&x)[2][W]) const {
+        const int g = lane >> 2, t = lane & 3;
+        // ranges of the 2 W groups over the 8 lanes of a position pair: each exchange halves what a lane holds, until
+        // lane g has one group's and works out its scale, which then goes to all
+        uint32_t rg[2 * W];
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                rg[e * W + w] = range_of(as_u32(__hmax2_nan(as_bf2(x[e][w].x), as_bf2(x[e][w].y))),
+                                         as_u32(__hmin2_nan(as_bf2(x[e][w].x), as_bf2(x[e][w].y))));
+#pragma unroll
+        for (int m = W, o = 16; m >= 1; m >>= 1, o >>= 1) {
+            const bool up = lane & o;
+#pragma unroll
+            for (int i = 0; i < m; i++) {
+                const uint32_t send = up ? rg[i] : rg[i + m], keep = up ? rg[i + m] : rg[i];
+                rg[i] = range_max(keep, __shfl_xor_sync(0xffffffffu, send, o));
+            }
+        }
+        if (W == 2) rg[0] = range_max(rg[0], __shfl_xor_sync(0xffffffffu, rg[0], 4));
+        const Quant mine = quant_of(rg[0]);
+        const uint32_t mine_sz = meta_bits(mine.s, mine.z);
+        Words<W> code, meta;
+        uint32_t sz[2][W], c[2][W], marks = 0;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int from = (e * W + w) * (16 / W) + t;
+                sz[e][w] = __shfl_sync(0xffffffffu, mine_sz, from);
+                const Quant q = quant_from(sz[e][w], __shfl_sync(0xffffffffu, mine.rinv, from));
+                const uint32_t pr[2] = {x[e][w].x, x[e][w].y};
+                c[e][w] = quant_pairs<2>(pr, q, marks);
+            }
+        }
+        const bool ok0 = ok(b * 8 + 2 * t), ok1 = ok(b * 8 + 2 * t + 1);
+        bool open = false;
+        if (marks & 1u) {
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    const uint32_t pr[2] = {x[e][w].x, x[e][w].y};
+                    open = (quant_marked<2>(pr, scale_of(sz[e][w]), zero_of(sz[e][w]), c[e][w]) && (e ? ok1 : ok0)) || open;
+                }
+        }
+#pragma unroll
+        for (int w = 0; w < W; w++) code.v[w] = __byte_perm(in_order(c[0][w]), in_order(c[1][w]), 0x5410);
+        uint8_t *half = u + (b & 7) / 4 * F::HALFB;
+        uint8_t *dst = half + F::CODES + (b & 3) * F::BLOCK + lane * 4 * W;
+        if (ok0 && ok1) {
+            st_words<W>(dst, code);
+        } else {  // one of the word's two positions belongs to this write: its halves only
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                if (ok0) reinterpret_cast<uint16_t *>(dst)[2 * w] = static_cast<uint16_t>(code.v[w]);
+                if (ok1) reinterpret_cast<uint16_t *>(dst)[2 * w + 1] = static_cast<uint16_t>(code.v[w] >> 16);
+            }
+        }
+        if (g == 0) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                if (!(e ? ok1 : ok0)) continue;
+#pragma unroll
+                for (int w = 0; w < W; w += 2) {
+                    meta.v[w / 2] = __byte_perm(sz[e][w], sz[e][w + 1], 0x5410);
+                    meta.v[W / 2 + w / 2] = __byte_perm(sz[e][w], sz[e][w + 1], 0x7632);
+                }
+                st_words<W>(half + F::VMETA + ((b & 3) * 8 + 2 * t + e) * F::ROW, meta);
+            }
+        }
+        return open;
+    }
+
+    // A block's codes once more, each by quant_exact, from the scales and zeros that stand in the page by now. For groups
+    // that real caches hardly have: short rather than fast.
+    __device__ __forceinline__ void exact(int b, int v) const {
+        __syncwarp();
+        uint8_t *half = u + (b & 7) / 4 * F::HALFB;
+        const int g = lane >> 2, t = lane & 3;
+        uint8_t *dst = half + v * F::CODES + (b & 3) * F::BLOCK + lane * 4 * W;
+#pragma unroll 1
+        for (int i = 0; i < 2 * W; i++) {  // 16-bit halves of the lane's words
+            const int w = i >> 1, e = i & 1;
+            const int p = b * 8 + (v ? 2 * t + e : g), c0 = 32 * w + (v ? 4 * g : 8 * t + e), step = v ? 1 : 2;
+            if (!ok(p)) continue;
+            const bf16 *row = reinterpret_cast<const bf16 *>(half + (v ? F::VMETA : F::KMETA) + p % HALF * F::ROW);
+            const float s = bf2f(row[w]), z = bf2f(row[W + w]);
+            uint32_t code = 0;
+#pragma unroll 1
+            for (int k = 0; k < 4; k++) code |= quant_exact(bf2f(src[p * pitch + c0 + k * step]), z, s) << (4 * k);
+            reinterpret_cast<uint16_t *>(dst)[i] = static_cast<uint16_t>(code);
+        }
+    }
+};
+
 // Bound by HBM: 512 bytes read and 160 written per position and kv head at hd 128. The lanes load row chunks in the order
 // of the block's words, so a block's 512 bytes of codes leave in one 16-byte store per lane.
 template <int HD>
-__global__ void __launch_bounds__(256) k_kv4_write(const bf16 *qkv, uint8_t *pool, const int *table, const int *start,
+__global__ void __launch_bounds__(256, 3) k_kv4_write(const bf16 *qkv, uint8_t *pool, const int *table, const int *start,
                                                    const int *count, int B, int rows, int nq, int nk, int npages,
                                                    int maxpages, int parts, int per) {
     using F = Fmt<HD>;
     constexpr int W = F::W;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31;
     const Part it(static_cast<long>(blockIdx.x) * 8 + (threadIdx.x >> 5), parts, nk);
     if (it.s >= B) return;
     const int p0 = start ? start[it.s] : 0, n = count ? min(count[it.s], rows) : rows;
@@ -210,139 +397,33 @@ __global__ void __launch_bounds__(256) k_kv4_write(const bf16 *qkv, uint8_t *poo
     uint8_t *u = unit_of(pool, table, it.s, b0 * 8, it.h, nk, npages, maxpages, F::UNIT);
     if (!u) return;
     const long pitch = static_cast<long>(nq + 2 * nk) * HD;
-    const bf16 *src = qkv + (static_cast<long>(it.s) * rows - p0) * pitch + (nq + it.v * nk + it.h) * HD;
-    auto ok = [&](int p) { return p >= p0 && p < p0 + n; };
-    if (it.v == 0) {  // K: lane 4g + t has channels 32w + 8t .. + 7 of position g
-        auto load = [&](int b, uint4 (&x)[W]) {
-            const int p = b * 8 + g;
-#pragma unroll
-            for (int w = 0; w < W; w++)
-                x[w] = ok(p) ? __ldcs(reinterpret_cast<const uint4 *>(src + p * pitch + 32 * w + 8 * t))
-                             : make_uint4(0, 0, 0, 0);
-        };
-        uint4 y[W];
-        load(first, y);
+    const WriteTo<HD> to{qkv + (static_cast<long>(it.s) * rows - p0) * pitch + (nq + it.v * nk + it.h) * HD, pitch, u, p0, n,
+                         lane};
+    unsigned again = 0;  // blocks, from the first, to be made again
+    if (it.v == 0) {
+        uint4 x[W], y[W];
+        to.load(first, y);
         for (int b = first; b <= last; b++) {
-            uint4 x[W];
 #pragma unroll
             for (int w = 0; w < W; w++) x[w] = y[w];
-            if (b < last) load(b + 1, y);
-            Words<W> code, meta;
-            uint32_t sz[W];
-#pragma unroll
-            for (int w = 0; w < W; w++) {
-                const uint32_t xu[4] = {x[w].x, x[w].y, x[w].z, x[w].w};
-                uint32_t mx = xu[0], mn = xu[0];
-#pragma unroll
-                for (int i = 1; i < 4; i++) {
-                    mx = as_u32(__hmax2_nan(as_bf2(mx), as_bf2(xu[i])));
-                    mn = as_u32(__hmin2_nan(as_bf2(mn), as_bf2(xu[i])));
-                }
-                uint32_t rg = range_of(mx, mn);
-                rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, 1));
-                rg = range_max(rg, __shfl_xor_sync(0xffffffffu, rg, 2));
-                const Quant q = quant_of(rg);
-                code.v[w] = quant_pairs<4>(xu, q);
-                sz[w] = meta_bits(q.s, q.z);
-            }
-            if (!ok(b * 8 + g)) continue;
-            uint8_t *half = u + (b & 7) / 4 * F::HALFB;
-            st_words<W>(half + (b & 3) * F::BLOCK + lane * 4 * W, code);
-            if (t == 0) {
-#pragma unroll
-                for (int w = 0; w < W; w += 2) {
-                    meta.v[w / 2] = __byte_perm(sz[w], sz[w + 1], 0x5410);
-                    meta.v[W / 2 + w / 2] = __byte_perm(sz[w], sz[w + 1], 0x7632);
-                }
-                st_words<W>(half + F::KMETA + ((b & 3) * 8 + g) * F::ROW, meta);
-            }
+            if (b < last) to.load(b + 1, y);
+            if (to.k_block(b, x)) again |= 1u << (b - first);
         }
-    } else {  // V: lane 4g + t has channels 32w + 4g .. + 3 of positions 2t and 2t + 1
-        auto load = [&](int b, uint2 (&x)[2][W]) {
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int p = b * 8 + 2 * t + e;
-#pragma unroll
-                for (int w = 0; w < W; w++)
-                    x[e][w] = ok(p) ? __ldcs(reinterpret_cast<const uint2 *>(src + p * pitch + 32 * w + 4 * g))
-                                    : make_uint2(0, 0);
-            }
-        };
-        uint2 y[2][W];
-        load(first, y);
+    } else {
+        uint2 x[2][W], y[2][W];
+        to.load(first, y);
         for (int b = first; b <= last; b++) {
-            uint2 x[2][W];
 #pragma unroll
             for (int e = 0; e < 2; e++)
 #pragma unroll
                 for (int w = 0; w < W; w++) x[e][w] = y[e][w];
-            if (b < last) load(b + 1, y);
-            Words<W> code, meta;
-            // ranges of the 2 W groups over the 8 lanes of a position pair: each exchange halves what a lane holds, until
-            // lane g has one group's and works out its scale, which then goes to all
-            uint32_t rg[2 * W];
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-#pragma unroll
-                for (int w = 0; w < W; w++)
-                    rg[e * W + w] = range_of(as_u32(__hmax2_nan(as_bf2(x[e][w].x), as_bf2(x[e][w].y))),
-                                             as_u32(__hmin2_nan(as_bf2(x[e][w].x), as_bf2(x[e][w].y))));
-#pragma unroll
-            for (int m = W, o = 16; m >= 1; m >>= 1, o >>= 1) {
-                const bool up = lane & o;
-#pragma unroll
-                for (int i = 0; i < m; i++) {
-                    const uint32_t send = up ? rg[i] : rg[i + m], keep = up ? rg[i + m] : rg[i];
-                    rg[i] = range_max(keep, __shfl_xor_sync(0xffffffffu, send, o));
-                }
-            }
-            if (W == 2) rg[0] = range_max(rg[0], __shfl_xor_sync(0xffffffffu, rg[0], 4));
-            const Quant mine = quant_of(rg[0]);
-            const uint32_t mine_sz = meta_bits(mine.s, mine.z);
-            uint32_t sz[2][W];
-#pragma unroll
-            for (int w = 0; w < W; w++) {
-                uint32_t n4[2];
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int from = (e * W + w) * (16 / W) + t;
-                    sz[e][w] = __shfl_sync(0xffffffffu, mine_sz, from);
-                    Quant q;
-                    q.s = __uint_as_float(sz[e][w] << 16);
-                    q.z = __uint_as_float(sz[e][w] & 0xffff0000u);
-                    q.rinv = __shfl_sync(0xffffffffu, mine.rinv, from);
-                    const uint32_t pr[2] = {x[e][w].x, x[e][w].y};
-                    const uint32_t c = quant_pairs<2>(pr, q);  // low half: channels 0, 2; high half: 1, 3
-                    n4[e] = (c & 0xfu) | (c >> 12 & 0xf0u) | (c << 4 & 0xf00u) | (c >> 8 & 0xf000u);
-                }
-                code.v[w] = __byte_perm(n4[0], n4[1], 0x5410);
-            }
-            uint8_t *half = u + (b & 7) / 4 * F::HALFB;
-            uint8_t *dst = half + F::CODES + (b & 3) * F::BLOCK + lane * 4 * W;
-            const bool ok0 = ok(b * 8 + 2 * t), ok1 = ok(b * 8 + 2 * t + 1);
-            if (ok0 && ok1) {
-                st_words<W>(dst, code);
-            } else {  // one of the word's two positions belongs to this write: its halves only
-#pragma unroll
-                for (int w = 0; w < W; w++) {
-                    if (ok0) reinterpret_cast<uint16_t *>(dst)[2 * w] = static_cast<uint16_t>(code.v[w]);
-                    if (ok1) reinterpret_cast<uint16_t *>(dst)[2 * w + 1] = static_cast<uint16_t>(code.v[w] >> 16);
-                }
-            }
-            if (g == 0) {
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    if (!(e ? ok1 : ok0)) continue;
-#pragma unroll
-                    for (int w = 0; w < W; w += 2) {
-                        meta.v[w / 2] = __byte_perm(sz[e][w], sz[e][w + 1], 0x5410);
-                        meta.v[W / 2 + w / 2] = __byte_perm(sz[e][w], sz[e][w + 1], 0x7632);
-                    }
-                    st_words<W>(half + F::VMETA + ((b & 3) * 8 + 2 * t + e) * F::ROW, meta);
-                }
-            }
+            if (b < last) to.load(b + 1, y);
+            if (to.v_block(b, x)) again |= 1u << (b - first);
         }
     }
+    again = __reduce_or_sync(0xffffffffu, again);
+    for (int b = first; again; b++, again >>= 1)
+        if (again & 1) to.exact(b, it.v);
 }
 
 // The 4 codes of nibbles 0..3 of a 16-bit half, as values rounded once to bf16 (s n is exact, the sum rounds once

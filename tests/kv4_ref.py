@@ -5,15 +5,28 @@ import torch
 PAGE = 64
 
 
+def minus(a, b):
+    """a - b as d + e exactly."""
+    d = a - b
+    bb = d - a
+    return d, (a - (d - bb)) + (-b - bb)
+
+
 def held(x):
-    """(codes, scales, zeros, values) of x [..., hd] in 64 bits; a group with a NaN or an infinity is NaN."""
+    """(codes, scales, zeros, values) of x [..., hd] in 64 bits; a group with a NaN or an infinity is NaN. Differences are
+    taken exactly: 2^-60 beside 1 is lost in 64 bits, and decides where what is left lies on a border."""
     g = x.double().unflatten(-1, (-1, 32))
     z, top = g.amin(-1), g.amax(-1)
-    want = (top - z) / 15
-    s = want.float().view(torch.int32) & -65536  # a bf16 at or below want, or the float's rounding up to one
-    low = s.view(torch.float32).double()
-    s = torch.where(low < want, (s + 65536).view(torch.float32).double(), low)
-    n = torch.round((g - z[..., None]) / torch.where(s > 0, s, 1.0)[..., None])
+    d, e = minus(top, z)
+    low = ((d / 15).float().view(torch.int32) & -65536).view(torch.float32)  # a bf16 at or below, or the next one
+    up = (low.view(torch.int32) + 65536).view(torch.float32).double()
+    low = low.double()
+    s = torch.where((15 * low > d) | ((15 * low == d) & (e <= 0)), low, up)
+    d, e = minus(g, z[..., None])
+    sc = torch.where(s > 0, s, 1.0)[..., None]
+    n = torch.floor(d / sc)
+    r = d - (n + 0.5) * sc
+    n = n + ((r > 0) | ((r == 0) & ((e > 0) | ((e == 0) & (n % 2 == 1)))))
     v = n * s[..., None] + z[..., None]
     bad = ~torch.isfinite(g).all(-1)
     v = torch.where(bad[..., None], torch.nan, v)

@@ -148,6 +148,47 @@ def test_write_of_ties_constants_and_extremes(cuda):
         assert torch.equal(got[0, 0, :n].nan_to_num(), want.nan_to_num())
 
 
+def special_groups():
+    """Groups in which the difference to the minimum is not exact in fp32, or a scale's reciprocal not a normal number:
+    0 on a border with tiny values beside it, minima tiny beside the scale, subnormal and constant groups."""
+    g = torch.Generator().manual_seed(11)
+    out = []
+    for m in range(15):  # -z = (m + 1/2) s: 0 lies on a border, s = 2
+        v = torch.empty(32).uniform_(-2.0 * m - 1, 29.0 - 2 * m, generator=g).double()
+        v[:8] = torch.tensor([2.0 ** -60, -(2.0 ** -60), 0.0, 2.0 ** -11, -(2.0 ** -11), 2.0 ** -13, -(2.0 ** -13), 1e-38])
+        v[30], v[31] = -2.0 * m - 1, 29.0 - 2 * m
+        out.append(v)
+    for e in (-4, -11, -12, -13, -20, -40, -100):  # borders of s = 2 behind a minimum that hides in rounding
+        out.append(torch.cat((torch.arange(1, 31, 2).double(), torch.arange(0, 32, 2).double(), -torch.tensor([2.0 ** e]))))
+    ramp = torch.arange(32).double() / 2
+    out += [ramp * 2.0 ** -e for e in (90, 100, 120, 127, 130, 133)] + [torch.zeros(32), torch.full((32,), -1e-30)]
+    return torch.stack(out).bfloat16()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_write_and_step_of_special_groups(cuda, hd):
+    W = hd // 32
+    x = special_groups()
+    x = torch.cat((x, x.flip(1), -x))
+    rows = torch.stack([x.roll(-3 * i, 0) for i in range(2 * W)], 1).reshape(x.shape[0], 2 * hd)  # k | v, one kv head
+    n = rows.shape[0]
+    pool = poisoned(-(-n // 64), 1, hd)
+    ops.kv4_write(rows.cuda().contiguous(), pool, i32([list(range(pool.shape[0]))]), None, None, 1, n, 0, 1, hd)
+    k, _, v, _ = ref.pool_values(pool.cpu(), 1, hd)
+    want = ref.held(rows.double())[3]
+    assert torch.equal(k.reshape(-1, hd)[:n], want[:, :hd]) and torch.equal(v.reshape(-1, hd)[:n], want[:, hd:])
+    # the same rows as the first positions of n takes, by the fused step
+    pool1, pool2 = poisoned(n, 1, hd), poisoned(n, 1, hd)
+    table, ones = i32([[i] for i in range(n)]), i32([1] * n)
+    qkv = torch.cat((randn(9, n, hd).cpu(), rows), 1).cuda().contiguous()
+    out, ws = torch.empty(n, hd, dtype=torch.bfloat16, device="cuda"), ops.decode_kv4_workspace(n, 1, 1, hd, 1)
+    held = torch.empty(n, 2 * hd, dtype=torch.bfloat16, device="cuda")
+    ops.attn_decode_kv4_step(qkv, pool1, out, ws, None, None, table, None, ones, n, 1, 1, hd, 0.1, held=held)
+    ops.kv4_write(qkv, pool2, table, None, None, n, 1, 1, 1, hd)
+    assert torch.equal(pool1, pool2)
+    assert torch.equal(held.cpu(), want.float().bfloat16())
+
+
 # ---- attention ----
 
 @pytest.mark.parametrize("nq,nk,hd", [(16, 2, 128), (8, 2, 64), (4, 4, 128), (7, 1, 64), (10, 2, 128), (3, 1, 128)])
