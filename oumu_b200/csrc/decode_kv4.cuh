@@ -804,66 +804,72 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
     // ---- segments that cross a boundary between warps, or the CTA's ends ----
     // The loops here are not unrolled: run once per launch, they cost their instruction fetches.
     constexpr int LPH = HD / 4;  // threads per head, 4 channels each
-    const int h = threadIdx.x / LPH, d4 = threadIdx.x % LPH;
-    auto store = [&](int id, float l, float4 o) {
+    const int d4 = threadIdx.x % LPH;
+    const unsigned mates = LPH == 32 ? 0xffffffffu : 0xffffu << (lane & 16);  // a head's threads in this warp
+    auto store = [&](int id, int h, float l, float4 o) {
         const float r = 1.f / l;
         uint2 u;
         u.x = pack_bf16x2(o.x * r, o.y * r);
         u.y = pack_bf16x2(o.z * r, o.w * r);
         *reinterpret_cast<uint2 *>(P.out + (static_cast<long>(id / nk) * P.nq + id % nk * G + h) * HD + 4 * d4) = u;
     };
-    auto add = [&](float f, float lw, float4 x, float &l, float4 &o) {
-        l = fmaf(f, lw, l);
-        o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
-    };
-    int crossing = 0;  // bit 0: the segment cut by the range's start, bit 1: by its end only, reaches into other CTAs
-    // boundaries that cut a segment for the first time, and those that cut the one before's again (a lane per boundary)
-    const int mine = lane <= nb ? cuts[lane].id : -1, left_one = __shfl_up_sync(0xffffffffu, mine, 1);
-    const bool again = lane > 0 && mine == left_one;
-    unsigned todo = __ballot_sync(0xffffffffu, mine >= 0 && !again);
-    const unsigned more = __ballot_sync(0xffffffffu, mine >= 0 && again);
+    // which cut segments reach into other CTAs. Bit 0: the one cut by the range's start, bit 1: by its end only
+    int crossing = cuts[0].id >= 0;
+    if (cuts[nb].id >= 0 && cuts[nb].start >= ta) crossing |= 2;
+    {
+        // boundaries that cut a segment for the first time, and those that cut the one before's again (a lane per boundary)
+        const int mine = lane <= nb ? cuts[lane].id : -1, left_one = __shfl_up_sync(0xffffffffu, mine, 1);
+        const bool again = lane > 0 && mine == left_one;
+        unsigned todo = __ballot_sync(0xffffffffu, mine >= 0 && !again);
+        const unsigned more = __ballot_sync(0xffffffffu, mine >= 0 && again);
+        constexpr int PER = GMAX / 2;  // a warp takes two heads of a segment
+        int done = 0;
 #pragma unroll 1
-    for (; todo; todo &= todo - 1) {
-        const int i = __ffs(todo) - 1;
-        const Cut x = cuts[i];
-        // the warps that have some of it: from the one before its first boundary to the one behind its last
-        const int first = max(i - 1, 0), last = min(i + __ffs(~(more >> i >> 1)) - 1, nb - 1);
-        const bool out = x.start < ta || x.end > tb;
-        if (out) crossing |= x.start < ta ? 1 : 2;
-        if (h >= G) continue;
-        auto at = [&](int w) {  // warp w's record of it: its last one if the segment goes on to the range's end
-            return x.end >= ta + parts.start(w + 1) ? reinterpret_cast<const float *>(sm + w * Y::RING)
-                                                    : reinterpret_cast<const float *>(sm + Y::FIRST) + w * Y::REC;
-        };
-        // the head's LPH threads take a record's reference and sum each
-        const unsigned mates = LPH == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
-        const bool has = first + d4 <= last;
-        const float m = has ? at(first + d4)[h] : -INFINITY;
-        float M = m;
+        for (int unit = warp;; unit += NW) {
+            for (; done < unit / PER; done++) todo &= todo - 1;
+            if (!todo) break;
+            const int i = __ffs(todo) - 1;
+            const Cut x = cuts[i];
+            // the warps that have some of it: from the one before its first boundary to the one behind its last
+            const int first = max(i - 1, 0), last = min(i + __ffs(~(more >> i >> 1)) - 1, nb - 1);
+            auto at = [&](int w) {  // warp w's record of it: its last one if the segment goes on to the range's end
+                return x.end >= ta + parts.start(w + 1) ? reinterpret_cast<const float *>(sm + w * Y::RING)
+                                                        : reinterpret_cast<const float *>(sm + Y::FIRST) + w * Y::REC;
+            };
+            const bool has = first + d4 <= last;  // the head's threads take a record's reference and sum each
+            const float *own = at(has ? first + d4 : first);
 #pragma unroll
-        for (int e = 1; e < 16; e <<= 1) M = fmaxf(M, __shfl_xor_sync(mates, M, e, 16));
-        M = __shfl_sync(mates, M, 0, LPH);
-        const float fm = fast_exp2(m - M);
-        float l = has ? fm * at(first + d4)[GMAX + h] : 0.f;
+            for (int hh = 0; hh < (LPH == 32 ? 2 : 1); hh++) {
+                const int h = unit % PER * 2 + (LPH == 32 ? hh : lane >> 4);
+                if (h >= G) continue;
+                const float m = has ? own[h] : -INFINITY;
+                float M = m;
 #pragma unroll
-        for (int e = 1; e < 16; e <<= 1) l += __shfl_xor_sync(mates, l, e, 16);
-        l = __shfl_sync(mates, l, 0, LPH);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int e = 1; e < 16; e <<= 1) M = fmaxf(M, __shfl_xor_sync(mates, M, e, 16));
+                M = __shfl_sync(mates, M, 0, LPH);
+                const float fm = fast_exp2(m - M);
+                float l = has ? fm * own[GMAX + h] : 0.f;
+#pragma unroll
+                for (int e = 1; e < 16; e <<= 1) l += __shfl_xor_sync(mates, l, e, 16);
+                l = __shfl_sync(mates, l, 0, LPH);
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
-        for (int w = first; w <= last; w++) {
-            const float f = __shfl_sync(mates, fm, w - first, LPH);
-            const float4 v = *reinterpret_cast<const float4 *>(at(w) + 2 * GMAX + h * HD + 4 * d4);
-            o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
-        }
-        if (!out) {
-            store(x.id, l, o);
-        } else {  // record 1 of a CTA is of a segment that starts in it
-            float *rec = P.part + (static_cast<long>(c) * 2 + (x.start >= ta)) * Y::REC;
-            if (d4 == 0) {
-                rec[h] = M;
-                rec[GMAX + h] = l;
+                for (int w = first; w <= last; w++) {
+                    const float f = __shfl_sync(mates, fm, w - first, LPH);
+                    const float4 v = *reinterpret_cast<const float4 *>(at(w) + 2 * GMAX + h * HD + 4 * d4);
+                    o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
+                }
+                if (x.start >= ta && x.end <= tb) {
+                    store(x.id, h, l, o);
+                } else {  // record 1 of a CTA is of a segment that starts in it
+                    float *rec = P.part + (static_cast<long>(c) * 2 + (x.start >= ta)) * Y::REC;
+                    if (d4 == 0) {
+                        rec[h] = M;
+                        rec[GMAX + h] = l;
+                    }
+                    *reinterpret_cast<float4 *>(rec + 2 * GMAX + h * HD + 4 * d4) = o;
+                }
             }
-            *reinterpret_cast<float4 *>(rec + 2 * GMAX + h * HD + 4 * d4) = o;
         }
     }
     if (!crossing) return;
@@ -877,6 +883,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         misc[1 + threadIdx.x] = done;
     }
     __syncthreads();
+    const int h = threadIdx.x / LPH;
 #pragma unroll 1
     for (int k = 0; k < 2; k++) {
         if (!(crossing >> k & 1) || !misc[1 + k] || h >= G) continue;
@@ -888,7 +895,6 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         };
         // up to 16 records' numerators on their way while the head's LPH threads take a record's reference and sum each
         constexpr int N = 16;
-        const unsigned mates = LPH == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
         float4 v[N];
 #pragma unroll
         for (int e = 0; e < N; e++) v[e] = cf + e <= cl ? numer(cf + e) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -920,7 +926,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         }
 #pragma unroll
         for (int e = 1; e < LPH; e <<= 1) l += __shfl_xor_sync(mates, l, e, LPH);
-        store(x.id, l, o);
+        store(x.id, h, l, o);
     }
 }
 
