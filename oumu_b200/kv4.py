@@ -11,13 +11,15 @@ from . import ops
 class KV4Cache:
     """`layers` layers of `npages` pages for B takes of up to maxlen positions. `lens` (int32 [B], device) holds the takes'
     lengths; a caller that advances its own on the device (oumu_step_end) passes it. Everything is enqueued on the
-    current stream and can be captured; nothing here waits for the GPU."""
+    current stream, without waiting for the GPU; calls to be captured take their takes as device tensors, not lists."""
 
     def __init__(self, layers, B, nq, nk, hd, npages, maxlen, device="cuda", lens=None):
         self.layers, self.B, self.nq, self.nk, self.hd, self.npages = layers, B, nq, nk, hd, npages
         self.maxpages = -(-maxlen // ops.KV4_PAGE)
         if layers < 1 or B < 1 or npages < 1 or maxlen < 1:
             raise ValueError("a cache has layers, takes, pages and positions")
+        if lens is not None and (lens.dtype is not torch.int32 or lens.numel() < B):
+            raise ValueError("lens: int32 [B]")
         dev = torch.device(device)
         i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)  # noqa: E731
         self.pools = torch.empty((layers, npages, ops.kv4_page_bytes(nk, hd)), dtype=torch.uint8, device=dev)

@@ -294,7 +294,7 @@ def kv4_page_bytes(nk, hd):
 
 
 def _kv4_check(pool, table, *ints, nk=0, hd=0, B=0):
-    """What the C entry points cannot see of tensors: types, layouts, sizes, the device."""
+    """What the C entry points cannot see of tensors: types, layouts, sizes, the device (which it returns)."""
     if pool.dtype is not torch.uint8 or not pool.is_contiguous():
         raise ValueError("pool: a contiguous uint8 tensor")
     if hd and (pool.dim() != 2 or hd not in HD_SUPPORTED or pool.shape[1] != nk * (2 * KV4_PAGE) * (hd * 5 // 8)):
@@ -305,6 +305,7 @@ def _kv4_check(pool, table, *ints, nk=0, hd=0, B=0):
     if pool.get_device() != dev:
         raise ValueError("the cache is not on the current device")
     _ints(dev, table, *ints)
+    return dev
 
 
 def _takes(n, *ts):
@@ -313,17 +314,22 @@ def _takes(n, *ts):
             raise ValueError("starts, counts and lengths: one per take")
 
 
-def _rows(t, n, what):
-    if t is not None and (t.dtype.itemsize != 2 or not t.is_contiguous() or t.numel() < n):
-        raise ValueError(f"{what}: contiguous 16-bit rows")
+def _rows(t, n, dev, what):
+    if t is not None and (t.dtype.itemsize != 2 or not t.is_contiguous() or t.numel() < n or t.get_device() != dev):
+        raise ValueError(f"{what}: contiguous 16-bit rows on the current device")
+
+
+def _workspace(t, dev):
+    if t.dtype is not torch.uint8 or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError("workspace: a contiguous uint8 tensor on the current device")
 
 
 def kv4_write(qkv, pool, table, start, count, B, rows, nq, nk, hd):
     """k and v of qkv rows s * rows + i, i < min(count[s], rows), quantised into take s's pages at start[s] + i
     (oumu_kv4_write; count None: every row, start None: from 0)."""
-    _kv4_check(pool, table, start, count, nk=nk, hd=hd, B=B)
+    dev = _kv4_check(pool, table, start, count, nk=nk, hd=hd, B=B)
     _takes(B, start, count)
-    _rows(qkv, B * rows * (nq + 2 * nk) * hd, "qkv")
+    _rows(qkv, B * rows * (nq + 2 * nk) * hd, dev, "qkv")
     _lib.call("oumu_kv4_write", _p(qkv), _p(pool), _p(table), _p(start), _p(count), B, rows, nq, nk, hd,
               pool.shape[0], table.shape[1], _stream())
 
@@ -332,10 +338,10 @@ def kv4_read(pool, table, lens, kc, vc, nk, hd, pos=None):
     """What the cache stands for of positions < lens[s] (or <= *pos), as bf16 slots kc, vc [B][nk][maxlen][hd]
     (oumu_kv4_read)."""
     B, maxlen = kc.shape[0], kc.shape[2]
-    _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
+    dev = _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
     _takes(B, lens)
-    _rows(kc, B * nk * maxlen * hd, "kc")
-    _rows(vc, B * nk * maxlen * hd, "vc")
+    _rows(kc, B * nk * maxlen * hd, dev, "kc")
+    _rows(vc, B * nk * maxlen * hd, dev, "vc")
     _lib.call("oumu_kv4_read", _p(pool), _p(table), _p(lens), _p(pos), _p(kc), _p(vc), B, nk, hd, pool.shape[0],
               table.shape[1], maxlen, _stream())
 
@@ -350,10 +356,11 @@ def decode_kv4_workspace(B, nq, nk, hd, maxpages, device=None):
 
 def attn_decode_kv4(qkv, pool, out, workspace, table, pos, lens, B, nq, nk, hd, scale):
     """attn_decode over the 4-bit paged cache (oumu_attn_decode_kv4). Lengths: lens[s] or *pos + 1."""
-    _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
+    dev = _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
     _takes(B, lens)
-    _rows(qkv, B * (nq + 2 * nk) * hd, "qkv")
-    _rows(out, B * nq * hd, "out")
+    _rows(qkv, B * (nq + 2 * nk) * hd, dev, "qkv")
+    _rows(out, B * nq * hd, dev, "out")
+    _workspace(workspace, dev)
     _lib.call("oumu_attn_decode_kv4", _p(qkv), _p(pool), _p(out), _p(workspace), workspace.numel(), _p(table), _p(pos),
               _p(lens), B, nq, nk, hd, pool.shape[0], table.shape[1], float(scale), _stream())
 
@@ -362,18 +369,20 @@ def attn_decode_kv4_step(qkv, pool, out, workspace, cos_t, sin_t, table, pos, le
     """One decode layer over the 4-bit paged cache in one launch: rope, quantisation and cache write of the newest
     position, then the attention (oumu_attn_decode_kv4_step). held: bf16 [B][2 nk hd], receives what the cache holds
     of the newest k and v."""
-    _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
+    dev = _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
     _takes(B, lens)
-    _rows(qkv, B * (nq + 2 * nk) * hd, "qkv")
-    _rows(out, B * nq * hd, "out")
-    _rows(held, B * 2 * nk * hd, "held")
+    _rows(qkv, B * (nq + 2 * nk) * hd, dev, "qkv")
+    _rows(out, B * nq * hd, dev, "out")
+    _workspace(workspace, dev)
+    _rows(held, B * 2 * nk * hd, dev, "held")
     rows = 0
     if cos_t is not None:
         rows = cos_t.shape[0]
         if (sin_t is None or cos_t.dtype is not torch.float32 or sin_t.dtype is not torch.float32
                 or cos_t.shape != (rows, hd // 2) or sin_t.shape != cos_t.shape
-                or not cos_t.is_contiguous() or not sin_t.is_contiguous()):
-            raise ValueError("cos_t and sin_t: contiguous fp32 [rows][hd / 2]")
+                or not cos_t.is_contiguous() or not sin_t.is_contiguous() or cos_t.get_device() != dev
+                or sin_t.get_device() != dev):
+            raise ValueError("cos_t and sin_t: contiguous fp32 [rows][hd / 2] on the current device")
     _lib.call("oumu_attn_decode_kv4_step", _p(qkv), _p(pool), _p(out), _p(held), _p(workspace), workspace.numel(),
               _p(cos_t), _p(sin_t), rows, _p(table), _p(pos), _p(lens), B, nq, nk, hd, pool.shape[0], table.shape[1],
               float(scale), _stream())
@@ -423,7 +432,7 @@ def pages_workspace(npages, device=None):
 
 def pages_compact(pools, table, ref, workspace, status):
     """Pages in use move to the front of the pools (oumu_pages_compact); status: [pages in use, pages moved]."""
-    _kv4_check(pools, table, ref, status)
+    _workspace(workspace, _kv4_check(pools, table, ref, status))
     if status.numel() < 2:
         raise ValueError("status: [2]")
     _lib.call("oumu_pages_compact", *_pools(pools, ref), _p(table), _p(ref), _p(workspace), workspace.numel(),

@@ -524,6 +524,95 @@ def test_tensors_the_entry_points_cannot_take_are_refused(cuda):
     call()
     for k in (dict(table=table.long()), dict(lens=ln.long()), dict(pool=pool[:, :-16]), dict(pool=pool.view(torch.int8)),
               dict(nk=1), dict(hd=64), dict(B=2), dict(qkv=qkv.float()), dict(out=out[:, ::2]), dict(table=table.cpu()),
-              dict(lens=ln.cpu())):
+              dict(lens=ln.cpu()), dict(qkv=qkv.cpu()), dict(out=out.cpu()), dict(ws=ws.cpu()), dict(ws=ws.float()),
+              dict(lens=ln[:0])):
         with pytest.raises(ValueError):
             call(**k)
+
+
+def test_a_small_workspace_runs_on_fewer_ctas(cuda):
+    nq, nk, hd, lens = 16, 2, 128, [900, 2500, 0, 77]
+    qkv, pool, rows, table, ln = attn_case(lens, nq, nk, hd, seed=70)
+    record = 2 * (16 + 8 * hd) * 4
+    for ctas in (1, 3):
+        ws = torch.zeros(256 + ctas * record, dtype=torch.uint8, device="cuda")
+        out = torch.empty(4, nq * hd, dtype=torch.bfloat16, device="cuda")
+        for _ in range(2):
+            ops.attn_decode_kv4(qkv, pool, out, ws, table, None, ln, 4, nq, nk, hd, hd ** -0.5)
+            check_attn(out, qkv, pool, rows, lens, nq, nk, hd)
+    with pytest.raises(RuntimeError):
+        ops.attn_decode_kv4(qkv, pool, out, ws[:256 + record - 16], table, None, ln, 4, nq, nk, hd, hd ** -0.5)
+
+
+def test_step_past_the_rotary_tables_is_reported(cuda):
+    nq, nk, hd, lens = 16, 2, 128, [100, 40]
+    qkv, pool, rows, table, ln = attn_case(lens, nq, nk, hd, seed=71)
+    cs, sn = (t.cuda() for t in ops.rotary_tables(64, hd))
+    ws = ops.decode_kv4_workspace(2, nq, nk, hd, table.shape[1])
+    out = [torch.empty(2, nq * hd, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ops.attn_decode_kv4_step(qkv, pool, out[0], ws, cs, sn, table, None, ln, 2, nq, nk, hd, hd ** -0.5)
+    assert ops.device_error(reset=True) == LENGTH
+    ops.attn_decode_kv4_step(qkv, pool, out[1], ws, cs, sn, table, None, i32([64, 40]), 2, nq, nk, hd, hd ** -0.5)
+    assert ops.device_error() == 0 and torch.equal(out[0], out[1])  # cut to what the tables hold
+
+
+def test_page_calls_captured_and_replayed(cuda):
+    """Free, fork, extend and compact in one graph, replayed as the takes grow, against the model."""
+    p = Model(5, 40, 6)
+    p.set_len(0, 150)
+    p.extend(0)
+    src, dst, gone = i32([0, 0]), i32([1, 3]), i32([3, 2, 3])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ops.pages_free(p.table, p.ref, p.lens, gone)
+        ops.pages_fork(p.pools, p.table, p.ref, p.lens, src, dst, p.status)
+        ops.pages_extend(p.table, p.ref, p.lens, 70, p.status)
+        ops.pages_compact(p.pools, p.table, p.ref, p.ws, p.status)
+    for grow in (0, 13, 64, 30):
+        if grow:
+            p.set_len(0, p.m.lens[0] + grow)
+            p.extend(0)
+        graph.replay()
+        for s in (3, 2, 3):
+            p.m.release(s)
+        p.m.fork([0, 0], [1, 3])
+        p.m.extend(70)
+        p.m.compact()
+        p.check()
+
+
+def test_step_with_programmatic_launches(cuda):
+    """A chain of steps and their page calls with programmatic dependent launches on gives what it gives without."""
+    nq, nk, hd, B, layers = 16, 2, 128, 6, 4
+    cs, sn = (t.cuda() for t in ops.rotary_tables(512, hd))
+    lens0 = [64, 1, 200, 127, 0, 333]
+    results = []
+    for pdl in (False, True):
+        pools = torch.zeros(layers, 40, ops.kv4_page_bytes(nk, hd), dtype=torch.uint8, device="cuda")
+        table, rf = torch.full((B, 8), -1, dtype=torch.int32, device="cuda"), i32([0] * 40)
+        lens, status = i32(lens0), i32([0, 0])
+        ws = ops.decode_kv4_workspace(B, nq, nk, hd, 8)
+        ops.pages_extend(table, rf, lens, 0, status)
+        kv = randn(80, layers, B * 333, 2 * nk * hd)
+        for l in range(layers):
+            ops.kv4_write(kv[l], pools[l], table, None, lens, B, 333, 0, nk, hd)
+        qkv = randn(81, B, (nq + 2 * nk) * hd)
+        outs = []
+        prev = ops.set_pdl(pdl)
+        try:
+            for _ in range(5):
+                lens.add_((lens > 0).int())
+                ops.pages_extend(table, rf, lens, 0, status)
+                x = qkv.clone()
+                for l in range(layers):
+                    out = torch.empty(B, nq * hd, dtype=torch.bfloat16, device="cuda")
+                    ops.attn_decode_kv4_step(x, pools[l], out, ws, cs, sn, table, None, lens, B, nq, nk, hd, hd ** -0.5)
+                    x = torch.cat((out, x[:, nq * hd:]), 1)  # the next layer's q is this one's output
+                    outs.append(out)
+        finally:
+            ops.set_pdl(prev)
+        results.append((torch.stack(outs), pools.clone()))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    assert ops.device_error() == 0
