@@ -258,10 +258,11 @@ int oumu_attn_decode_kv4(const void *qkv, const void *pool, void *out, void *wor
 
 /*
  * oumu_attn_decode_step over the 4-bit cache: in one launch, every take's newest position (lens[s] - 1, or *pos) has
- * its k rotated (cos_t, sin_t [rot_rows][hd / 2]; NULL for no rope; a length above rot_rows is one the table does
- * not hold), k and v quantised into its page, and its q rotated and attended over positions up to and including it, all as the cache stands for them: the output of
- * oumu_rope, oumu_kv4_write and oumu_attn_decode_kv4, bit for bit. qkv is not modified. held: bf16 [B][2 nk hd] or
- * NULL, receives what the cache now holds of the newest k (heads), then v; zeros for a take of length 0.
+ * its k rotated (cos_t, sin_t [rot_rows][hd / 2]; NULL for no rope; a length above rot_rows counts as one the table
+ * does not hold), k and v quantised into its page, and its q rotated and attended over positions up to and including
+ * it, all as the cache stands for them: the output of oumu_rope, oumu_kv4_write and oumu_attn_decode_kv4, bit for bit.
+ * qkv is not modified. held: bf16 [B][2 nk hd] or NULL, receives what the cache now holds of the newest k (heads),
+ * then v; zeros for a take of length 0.
  */
 int oumu_attn_decode_kv4_step(const void *qkv, void *pool, void *out, void *held, void *workspace,
                               size_t workspace_bytes, const float *cos_t, const float *sin_t, int rot_rows,

@@ -966,11 +966,12 @@ int launch_decode_kv4(bool fused, const d4::Params &P, size_t ws_bytes, int sms,
                      dim3(NW * 32), d4::Lay<HD, NW>::bytes(P.B), st, P));
     return OUMU_OK;
 }
-// 12 warps where full tables would give 8 warps an SM 16 tiles each, or more (lengths are known on the device only).
+// 12 warps where full tables would give 8 warps an SM 10 tiles each, or more (lengths are known on the device only). 8 | 12
+// warps: 256 takes of up to 4096 positions 53.3 | 49.2 us, 64 takes 21.9 | 21.3, 32 takes 17.3 | 18.3, one of 512 8.4 | 9.5.
 template <int HD>
 int launch_decode_kv4(bool fused, const d4::Params &P, size_t ws_bytes, int sms, cudaStream_t st) {
     const long tiles = static_cast<long>(P.B) * P.nk * P.maxpages * (kv4::PAGE / d4::TP<HD>);
-    return tiles >= 16L * 8 * sms ? launch_decode_kv4<HD, 12>(fused, P, ws_bytes, sms, st)
+    return tiles >= 10L * 8 * sms ? launch_decode_kv4<HD, 12>(fused, P, ws_bytes, sms, st)
                                   : launch_decode_kv4<HD, 8>(fused, P, ws_bytes, sms, st);
 }
 
