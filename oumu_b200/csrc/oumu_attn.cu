@@ -932,6 +932,8 @@ namespace {
 int paged_limits(int B, int npages, int maxpages) {
     if (B < 1 || npages < 1 || maxpages < 1) return OUMU_ERR_INVALID;
     if (B > pg::BMAX || static_cast<long>(maxpages) * kv4::PAGE >= (1L << 31)) return OUMU_ERR_UNSUPPORTED;
+    // page and entry numbers are counted in int, page numbers up to a planning block's 4096 past the last
+    if (npages > (1 << 30) || static_cast<long>(B) * maxpages >= (1L << 31)) return OUMU_ERR_UNSUPPORTED;
     return OUMU_OK;
 }
 
@@ -1143,7 +1145,7 @@ int oumu_pages_free(int *table, int *ref, int *lens, const int *takes, int n, in
     return OUMU_OK;
 }
 
-size_t oumu_pages_workspace(int npages) { return npages < 1 ? 0 : pg::Plan::bytes(npages); }
+size_t oumu_pages_workspace(int npages) { return paged_limits(1, npages, 1) ? 0 : pg::Plan::bytes(npages); }
 
 int oumu_pages_compact(void *pools, long layer_stride, int layers, long page_bytes, int *table, int *ref,
                        void *workspace, size_t workspace_bytes, int *status, int B, int npages, int maxpages,

@@ -315,8 +315,8 @@ def _takes(n, *ts):
 
 
 def _rows(t, n, dev, what):
-    if t is not None and (t.dtype.itemsize != 2 or not t.is_contiguous() or t.numel() < n or t.get_device() != dev):
-        raise ValueError(f"{what}: contiguous 16-bit rows on the current device")
+    if t is not None and (t.dtype is not torch.bfloat16 or not t.is_contiguous() or t.numel() < n or t.get_device() != dev):
+        raise ValueError(f"{what}: contiguous bf16 rows on the current device")
 
 
 def _workspace(t, dev):

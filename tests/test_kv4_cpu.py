@@ -95,6 +95,18 @@ def test_page_refusals(lib):
     assert lib.oumu_pages_compact(P, 128, 1, 16, P, P, ODD, need, P, 4, 8, 8, None) == INVALID
 
 
+def test_refusals_of_tables_and_pools_that_int_cannot_count(lib):
+    for npages, B, maxpages in (((1 << 30) + 1, 4, 8), ((1 << 31) - 1, 1, 8), (8, 4096, 1 << 19), (8, 64, 1 << 25)):
+        assert lib.oumu_pages_extend(P, P, P, 0, P, B, npages, maxpages, None) == UNSUPPORTED
+        assert lib.oumu_pages_fork(P, 0, 1, 16, P, P, P, P, P, 1, P, B, npages, maxpages, None) == UNSUPPORTED
+        assert lib.oumu_pages_free(P, P, P, P, 1, B, npages, maxpages, None) == UNSUPPORTED
+        assert lib.oumu_pages_compact(P, 1 << 40, 1, 16, P, P, P, 1 << 40, P, B, npages, maxpages, None) == UNSUPPORTED
+        assert lib.oumu_kv4_write(P, P, P, None, None, B, 4, 16, 2, 128, npages, maxpages, None) == UNSUPPORTED
+        assert lib.oumu_kv4_read(P, P, P, None, P, P, B, 2, 128, npages, maxpages, 64, None) == UNSUPPORTED
+    assert lib.oumu_pages_workspace((1 << 30) + 1) == 0
+    assert lib.oumu_pages_workspace(1 << 30) == 4 * (4 + 2 * ((1 << 29) + 1) + (1 << 30))
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("kind", ["k", "v"])
 def test_every_code_has_a_place_of_its_own(hd, kind):

@@ -515,6 +515,32 @@ def test_two_streams_with_their_own_workspaces(cuda):
     assert all(torch.equal(o, w) for o, w in zip(outs, want))
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("maxpages", [1, 4])  # 8 warps, and 12
+def test_the_most_takes(cuda, hd, maxpages):
+    B, nq, nk = 4096, 2, 1
+    r = random.Random(maxpages)
+    lens = [r.choice((0, 1, 7, 33, 64 * maxpages)) for _ in range(B)]
+    qkv, pool, rows, table, ln = attn_case(lens, nq, nk, hd, seed=maxpages)
+    out = run_attn(qkv, pool, table, ln, B, nq, nk, hd)
+    some = sorted(r.sample(range(B), 40)) + [B - 1]
+    check_attn(out[some], qkv[some], pool, [rows[i] for i in some], [lens[i] for i in some], nq, nk, hd)
+    with pytest.raises(ValueError):
+        ops.decode_kv4_workspace(B + 1, nq, nk, hd, maxpages)
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.int16])
+def test_rows_of_another_16_bit_type_are_refused(cuda, t):
+    qkv, pool, rows, table, ln = attn_case([70], 16, 2, 128)
+    out, ws = torch.empty(1, 2048, dtype=torch.bfloat16, device="cuda"), ops.decode_kv4_workspace(1, 16, 2, 128, 2)
+    with pytest.raises(ValueError):
+        ops.attn_decode_kv4(qkv.view(t), pool, out, ws, table, None, ln, 1, 16, 2, 128, 0.1)
+    with pytest.raises(ValueError):
+        ops.attn_decode_kv4(qkv, pool, out.view(t), ws, table, None, ln, 1, 16, 2, 128, 0.1)
+    with pytest.raises(ValueError):
+        ops.kv4_write(qkv.view(t), pool, table, None, None, 1, 1, 16, 2, 128)
+
+
 def test_tensors_the_entry_points_cannot_take_are_refused(cuda):
     nq, nk, hd = 16, 2, 128
     qkv, pool, rows, table, ln = attn_case([70], nq, nk, hd)
