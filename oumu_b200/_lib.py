@@ -98,7 +98,8 @@ def check(fn, status):
         raise OumuError(fn, status)
 
 
-# entry-point calls made through call() (each launches at most one kernel); read by the benchmark to count launches
+# entry-point calls made through call() (each launches at most one kernel, oumu_pages_fork and oumu_pages_compact
+# two); read by the benchmark to count launches
 CALLS = [0]
 
 

@@ -10,15 +10,16 @@ import torch
 from . import _lib
 
 HD_SUPPORTED = (64, 128)
+_BF16 = (torch.bfloat16, torch.int16, torch.uint16)  # types of bf16 buffers
 
 
 def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream():
+def _stream(dev=None):
     # the current stream's handle without building a Stream object around it (0.3 us a call instead of 3.3)
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev is None else dev)
 
 
 def _ints(dev, *ts):
@@ -294,18 +295,20 @@ def kv4_page_bytes(nk, hd):
 
 
 def _kv4_check(pool, table, *ints, nk=0, hd=0, B=0):
-    """What the C entry points cannot see of tensors: types, layouts, sizes, the device (which it returns)."""
+    """What the C entry points cannot see of tensors: types, layouts, sizes, the device. Returns the device, the pool's
+    shape and maxpages."""
     if pool.dtype is not torch.uint8 or not pool.is_contiguous():
         raise ValueError("pool: a contiguous uint8 tensor")
-    if hd and (pool.dim() != 2 or hd not in HD_SUPPORTED or pool.shape[1] != nk * (2 * KV4_PAGE) * (hd * 5 // 8)):
+    shape, rows = pool.shape, table.shape
+    if hd and (len(shape) != 2 or hd not in HD_SUPPORTED or shape[1] != nk * (2 * KV4_PAGE) * (hd * 5 // 8)):
         raise ValueError("pool: [npages][kv4_page_bytes(nk, hd)]")
-    if table.dim() != 2 or table.shape[0] < B:
+    if len(rows) != 2 or rows[0] < B:
         raise ValueError("table: [B][maxpages]")
     dev = torch.cuda.current_device()
     if pool.get_device() != dev:
         raise ValueError("the cache is not on the current device")
     _ints(dev, table, *ints)
-    return dev
+    return dev, shape, rows[1]
 
 
 def _takes(n, *ts):
@@ -315,8 +318,8 @@ def _takes(n, *ts):
 
 
 def _rows(t, n, dev, what):
-    if t is not None and (t.dtype is not torch.bfloat16 or not t.is_contiguous() or t.numel() < n or t.get_device() != dev):
-        raise ValueError(f"{what}: contiguous bf16 rows on the current device")
+    if t is not None and (t.dtype not in _BF16 or not t.is_contiguous() or t.numel() < n or t.get_device() != dev):
+        raise ValueError(f"{what}: contiguous bf16 rows (or their bits as 16-bit integers) on the current device")
 
 
 def _workspace(t, dev):
@@ -327,23 +330,23 @@ def _workspace(t, dev):
 def kv4_write(qkv, pool, table, start, count, B, rows, nq, nk, hd):
     """k and v of qkv rows s * rows + i, i < min(count[s], rows), quantised into take s's pages at start[s] + i
     (oumu_kv4_write; count None: every row, start None: from 0)."""
-    dev = _kv4_check(pool, table, start, count, nk=nk, hd=hd, B=B)
+    dev, shape, maxpages = _kv4_check(pool, table, start, count, nk=nk, hd=hd, B=B)
     _takes(B, start, count)
     _rows(qkv, B * rows * (nq + 2 * nk) * hd, dev, "qkv")
     _lib.call("oumu_kv4_write", _p(qkv), _p(pool), _p(table), _p(start), _p(count), B, rows, nq, nk, hd,
-              pool.shape[0], table.shape[1], _stream())
+              shape[0], maxpages, _stream(dev))
 
 
 def kv4_read(pool, table, lens, kc, vc, nk, hd, pos=None):
     """What the cache stands for of positions < lens[s] (or <= *pos), as bf16 slots kc, vc [B][nk][maxlen][hd]
     (oumu_kv4_read)."""
-    B, maxlen = kc.shape[0], kc.shape[2]
-    dev = _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
+    B, _, maxlen, _ = kc.shape
+    dev, shape, maxpages = _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
     _takes(B, lens)
     _rows(kc, B * nk * maxlen * hd, dev, "kc")
     _rows(vc, B * nk * maxlen * hd, dev, "vc")
-    _lib.call("oumu_kv4_read", _p(pool), _p(table), _p(lens), _p(pos), _p(kc), _p(vc), B, nk, hd, pool.shape[0],
-              table.shape[1], maxlen, _stream())
+    _lib.call("oumu_kv4_read", _p(pool), _p(table), _p(lens), _p(pos), _p(kc), _p(vc), B, nk, hd, shape[0],
+              maxpages, maxlen, _stream(dev))
 
 
 def decode_kv4_workspace(B, nq, nk, hd, maxpages, device=None):
@@ -356,20 +359,20 @@ def decode_kv4_workspace(B, nq, nk, hd, maxpages, device=None):
 
 def attn_decode_kv4(qkv, pool, out, workspace, table, pos, lens, B, nq, nk, hd, scale):
     """attn_decode over the 4-bit paged cache (oumu_attn_decode_kv4). Lengths: lens[s] or *pos + 1."""
-    dev = _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
+    dev, shape, maxpages = _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
     _takes(B, lens)
     _rows(qkv, B * (nq + 2 * nk) * hd, dev, "qkv")
     _rows(out, B * nq * hd, dev, "out")
     _workspace(workspace, dev)
     _lib.call("oumu_attn_decode_kv4", _p(qkv), _p(pool), _p(out), _p(workspace), workspace.numel(), _p(table), _p(pos),
-              _p(lens), B, nq, nk, hd, pool.shape[0], table.shape[1], float(scale), _stream())
+              _p(lens), B, nq, nk, hd, shape[0], maxpages, float(scale), _stream(dev))
 
 
 def attn_decode_kv4_step(qkv, pool, out, workspace, cos_t, sin_t, table, pos, lens, B, nq, nk, hd, scale, held=None):
     """One decode layer over the 4-bit paged cache in one launch: rope, quantisation and cache write of the newest
     position, then the attention (oumu_attn_decode_kv4_step). held: bf16 [B][2 nk hd], receives what the cache holds
     of the newest k and v."""
-    dev = _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
+    dev, shape, maxpages = _kv4_check(pool, table, lens, pos, nk=nk, hd=hd, B=B)
     _takes(B, lens)
     _rows(qkv, B * (nq + 2 * nk) * hd, dev, "qkv")
     _rows(out, B * nq * hd, dev, "out")
@@ -384,56 +387,60 @@ def attn_decode_kv4_step(qkv, pool, out, workspace, cos_t, sin_t, table, pos, le
                 or sin_t.get_device() != dev):
             raise ValueError("cos_t and sin_t: contiguous fp32 [rows][hd / 2] on the current device")
     _lib.call("oumu_attn_decode_kv4_step", _p(qkv), _p(pool), _p(out), _p(held), _p(workspace), workspace.numel(),
-              _p(cos_t), _p(sin_t), rows, _p(table), _p(pos), _p(lens), B, nq, nk, hd, pool.shape[0], table.shape[1],
-              float(scale), _stream())
+              _p(cos_t), _p(sin_t), rows, _p(table), _p(pos), _p(lens), B, nq, nk, hd, shape[0], maxpages,
+              float(scale), _stream(dev))
 
 
-def _pools(pools, ref):
-    if pools.dim() != 3 or ref.numel() != pools.shape[1]:
+def _pools(pools, shape, ref):
+    if len(shape) != 3 or ref.numel() != shape[1]:
         raise ValueError("pools: [layers][npages][page bytes], ref: [npages]")
-    return _p(pools), pools.stride(0), pools.shape[0], pools.shape[2]
+    return _p(pools), shape[1] * shape[2], shape[0], shape[2]
 
 
 def pages_extend(table, ref, lens, extra, status):
     """Every take that holds positions gets the pages it lacks for lens[s] + extra of them (oumu_pages_extend);
     status[0]: pages missing."""
-    _ints(torch.cuda.current_device(), table, ref, lens, status)
-    if table.dim() != 2 or lens.numel() < table.shape[0] or status.numel() < 1:
+    dev, rows = torch.cuda.current_device(), table.shape
+    _ints(dev, table, ref, lens, status)
+    if len(rows) != 2 or lens.numel() < rows[0] or status.numel() < 1:
         raise ValueError("table: [B][maxpages], lens: [B], status: [1]")
-    _lib.call("oumu_pages_extend", _p(table), _p(ref), _p(lens), extra, _p(status), table.shape[0], ref.numel(),
-              table.shape[1], _stream())
+    _lib.call("oumu_pages_extend", _p(table), _p(ref), _p(lens), extra, _p(status), rows[0], ref.numel(), rows[1],
+              _stream(dev))
 
 
 def pages_fork(pools, table, ref, lens, src, dst, status):
     """Take dst[i] continues where take src[i] is: shared full pages, a copy of the last one (oumu_pages_fork);
     status[0]: pages missing."""
-    _kv4_check(pools, table, ref, lens, src, dst, status)
-    if lens.numel() < table.shape[0] or src.numel() != dst.numel() or status.numel() < 1:
+    dev, shape, maxpages = _kv4_check(pools, table, ref, lens, src, dst, status)
+    B, n = len(table), src.numel()
+    if lens.numel() < B or n != dst.numel() or status.numel() < 1:
         raise ValueError("lens: [B], src and dst: one take each per pair, status: [1]")
-    _lib.call("oumu_pages_fork", *_pools(pools, ref), _p(table), _p(ref), _p(lens), _p(src), _p(dst), src.numel(),
-              _p(status), table.shape[0], ref.numel(), table.shape[1], _stream())
+    _lib.call("oumu_pages_fork", *_pools(pools, shape, ref), _p(table), _p(ref), _p(lens), _p(src), _p(dst), n,
+              _p(status), B, shape[1], maxpages, _stream(dev))
 
 
 def pages_free(table, ref, lens, takes):
     """The takes give their pages back and are empty (oumu_pages_free)."""
-    _ints(torch.cuda.current_device(), table, ref, lens, takes)
+    dev = torch.cuda.current_device()
+    _ints(dev, table, ref, lens, takes)
     if table.dim() != 2 or lens.numel() < table.shape[0]:
         raise ValueError("table: [B][maxpages], lens: [B]")
     _lib.call("oumu_pages_free", _p(table), _p(ref), _p(lens), _p(takes), takes.numel(), table.shape[0], ref.numel(),
-              table.shape[1], _stream())
+              table.shape[1], _stream(dev))
 
 
 def pages_workspace(npages, device=None):
     n = int(_lib.load().oumu_pages_workspace(npages))
     if n == 0:
-        raise ValueError("a pool has at least one page")
+        raise ValueError("a pool has at least one page, and 2^30 at most")
     return torch.empty(n, dtype=torch.uint8, device=device or "cuda")
 
 
 def pages_compact(pools, table, ref, workspace, status):
     """Pages in use move to the front of the pools (oumu_pages_compact); status: [pages in use, pages moved]."""
-    _workspace(workspace, _kv4_check(pools, table, ref, status))
+    dev, shape, maxpages = _kv4_check(pools, table, ref, status)
+    _workspace(workspace, dev)
     if status.numel() < 2:
         raise ValueError("status: [2]")
-    _lib.call("oumu_pages_compact", *_pools(pools, ref), _p(table), _p(ref), _p(workspace), workspace.numel(),
-              _p(status), table.shape[0], ref.numel(), table.shape[1], _stream())
+    _lib.call("oumu_pages_compact", *_pools(pools, shape, ref), _p(table), _p(ref), _p(workspace), workspace.numel(),
+              _p(status), len(table), shape[1], maxpages, _stream(dev))

@@ -529,16 +529,19 @@ def test_the_most_takes(cuda, hd, maxpages):
         ops.decode_kv4_workspace(B + 1, nq, nk, hd, maxpages)
 
 
-@pytest.mark.parametrize("t", [torch.float16, torch.int16])
-def test_rows_of_another_16_bit_type_are_refused(cuda, t):
+def test_rows_may_be_bf16_bits_but_no_other_16_bit_type(cuda):
     qkv, pool, rows, table, ln = attn_case([70], 16, 2, 128)
     out, ws = torch.empty(1, 2048, dtype=torch.bfloat16, device="cuda"), ops.decode_kv4_workspace(1, 16, 2, 128, 2)
+    bits = torch.zeros_like(out, dtype=torch.int16)
+    ops.attn_decode_kv4(qkv, pool, out, ws, table, None, ln, 1, 16, 2, 128, 0.1)
+    ops.attn_decode_kv4(qkv.view(torch.int16), pool, bits, ws, table, None, ln, 1, 16, 2, 128, 0.1)
+    assert torch.equal(out.view(torch.int16), bits)
     with pytest.raises(ValueError):
-        ops.attn_decode_kv4(qkv.view(t), pool, out, ws, table, None, ln, 1, 16, 2, 128, 0.1)
+        ops.attn_decode_kv4(qkv.view(torch.float16), pool, out, ws, table, None, ln, 1, 16, 2, 128, 0.1)
     with pytest.raises(ValueError):
-        ops.attn_decode_kv4(qkv, pool, out.view(t), ws, table, None, ln, 1, 16, 2, 128, 0.1)
+        ops.attn_decode_kv4(qkv, pool, out.view(torch.float16), ws, table, None, ln, 1, 16, 2, 128, 0.1)
     with pytest.raises(ValueError):
-        ops.kv4_write(qkv.view(t), pool, table, None, None, 1, 1, 16, 2, 128)
+        ops.kv4_write(qkv.view(torch.float16), pool, table, None, None, 1, 1, 16, 2, 128)
 
 
 def test_tensors_the_entry_points_cannot_take_are_refused(cuda):
