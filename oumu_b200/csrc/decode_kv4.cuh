@@ -2,8 +2,8 @@
 // position's rope, quantisation and cache write in the same launch.
 //
 // Measured (one B200, back to back in a graph, 16 q and 2 kv heads of 128): 256 takes of 330..4096 positions, 184 MB,
-// 49.2 us (3.7 TB/s; the copies alone take 32); 64 takes 21.3 us; 32 takes 17.3; 2 takes of 65536 positions 21.3; one of
-// 512 8.4. Long caches stream at 6.3 TB/s, the rest is fixed: 3 us to the first tile, 3 to 4 from a CTA's last tile to
+// 49.4 us (3.7 TB/s; the copies alone take 32); 64 takes 21.0 us; 32 takes 17.5; 2 takes of 65536 positions 21.0; one of
+// 512 8.3. Long caches stream at 6.3 TB/s, the rest is fixed: 3 us to the first tile, 3 to 4 from a CTA's last tile to
 // the end (merge, counter, the last one's sum), 2 of launch, and what the warps' ends differ by.
 //
 // The mathematics. With value = s n + z for each group of 32 channels,
@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         return;
     }
     const Parts parts(tb - ta, NW);
-    // by way of a shuffle: the loop then takes 12 registers fewer (long caches 6.26 TB/s, 6.05 without)
+    // by way of a shuffle: the loop then takes 3 to 12 registers fewer (long caches 6.26 TB/s, 6.05 without)
     const int bound = ta + parts.start(warp + (lane & 1));
     const int wa = __shfl_sync(0xffffffffu, bound, 0), wb = __shfl_sync(0xffffffffu, bound, 1), n = wb - wa;
 
