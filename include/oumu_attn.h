@@ -219,7 +219,7 @@ int oumu_attn_prefill_kv(const void *qkv, void *out, void *kc, void *vc, int T, 
  * What is read on the device is checked there: a position no table entry has a page for, an entry outside
  * [0, npages), a take outside [0, B) sets OUMU_DEVERR_PAGE (4), a length or position outside the table's
  * [0, 64 maxpages] sets OUMU_DEVERR_LENGTH (2) in the word of oumu_device_error; nothing is read or written out of
- * range, and the outputs of the takes concerned are unspecified. A page that more than one take holds (ref > 1) must
+ * range, no page is written for the takes concerned, and their outputs are unspecified. A page that more than one take holds (ref > 1) must
  * not be written: oumu_pages_fork shares full pages only, so a take that only grows never does.
  * B <= 4096, 64 * maxpages < 2^31, B * maxpages < 2^31 and npages <= 2^30 throughout, else OUMU_ERR_UNSUPPORTED.
  */

@@ -451,8 +451,8 @@ struct State {
 };
 
 // Fused form: the newest position's k (rotated) and v, quantised by the warp that has the segment's last tile. Lane l has
-// channels 4l .. 4l + 3. `make` writes them into the take's page (and `held`) as soon as q arrives; `patch` into the
-// copy of that half in shared memory, which was on its way already.
+// channels 4l .. 4l + 3. `make` writes them into the take's page (`half`; null: not at all) and `held` as soon as q
+// arrives; `patch` into the copy of that half in shared memory, which was on its way already.
 template <int HD>
 struct Newest {
     static constexpr int W = Fmt<HD>::W;
@@ -528,7 +528,7 @@ struct Newest {
             }
             meta[kv] = kv4::meta_bits(q.s, q.z);
         }
-        patch(half, p % HALF, lane);
+        if (half) patch(half, p % HALF, lane);
     }
 };
 
@@ -752,10 +752,14 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
             S.clear();
             const bool ends = stop == k + T - j;  // its last tile is this warp's
             if (FUSED && ends) {
+                // a length that take_len has cut is not this position's: what the page holds there, for other takes too,
+                // stays
                 const int page = P.table[static_cast<long>(s) * P.maxpages + (L - 1) / kv4::PAGE];
-                if (page >= 0 && page < P.npages)
-                    N.make(P, s, kh, L - 1, lane,
-                           P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT + (L - 1) % kv4::PAGE / HALF * F::HALFB);
+                const bool write = page >= 0 && page < P.npages && (P.lens ? P.lens[s] : *P.pos + 1) == L;
+                N.make(P, s, kh, L - 1, lane,
+                       write ? P.pool + (static_cast<long>(page) * nk + kh) * F::UNIT +
+                                   (L - 1) % kv4::PAGE / HALF * F::HALFB
+                             : nullptr);
             }
             for (; issued < ST && issued < n; issued++) issue(issued);  // behind every warp's first tile
             int left = L - j * TP;  // positions from this tile on
