@@ -67,6 +67,15 @@ int oumu_step_end(const void *stop_logits, const void *patch, void *patches, int
                   int min_len, int max_steps, oumu_stream_t stream);
 
 /*
+ * oumu_step_end for takes on pages (oumu_attn.h): lens[s] += 1 only where lens[s] > 0 and take s had not stopped before
+ * this step. A stopped take keeps its length, so it takes no more pages and what it held when it stopped is not written
+ * again (each later step writes its position lens[s] - 1, the one behind them); a take that holds nothing stays empty.
+ * lens is not NULL.
+ */
+int oumu_step_end_live(const void *stop_logits, const void *patch, void *patches, int *stop, int *ctr, int *lens, int B,
+                       int min_len, int max_steps, oumu_stream_t stream);
+
+/*
  * The decoding loop as one graph launch, with the stop test on the device: Engine::decode (src/model.rs:777-796)
  * replays the step graph and reads `stop` back after every step; this runs
  *     while (ctr[1] < max_steps && some stop[s] < 0 for s < B) { step; }

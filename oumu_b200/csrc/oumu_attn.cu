@@ -1239,14 +1239,28 @@ int oumu_cfg_euler(void *x, const void *out, int B, int seq, int first, float dt
     return OUMU_OK;
 }
 
-int oumu_step_end(const void *stop_logits, const void *patch, void *patches, int *stop, int *ctr, int *lens, int B,
-                  int min_len, int max_steps, oumu_stream_t stream) {
+namespace {
+int step_end(bool live, const void *stop_logits, const void *patch, void *patches, int *stop, int *ctr, int *lens, int B,
+             int min_len, int max_steps, oumu_stream_t stream) {
     if (!stop_logits || !patch || !patches || !stop || !ctr || B < 0 || max_steps < 1) return OUMU_ERR_INVALID;
     if (!aligned16(patch) || !aligned16(patches)) return OUMU_ERR_INVALID;
-    glue::k_step_end<<<1, 256, 0, stream>>>(static_cast<const bf16 *>(stop_logits), static_cast<const bf16 *>(patch),
-                                            static_cast<bf16 *>(patches), stop, ctr, lens, B, min_len, max_steps);
+    auto kern = live ? glue::k_step_end<true> : glue::k_step_end<false>;
+    kern<<<1, 256, 0, stream>>>(static_cast<const bf16 *>(stop_logits), static_cast<const bf16 *>(patch),
+                                static_cast<bf16 *>(patches), stop, ctr, lens, B, min_len, max_steps);
     OUMU_CK(cudaGetLastError());
     return OUMU_OK;
+}
+}  // namespace
+
+int oumu_step_end(const void *stop_logits, const void *patch, void *patches, int *stop, int *ctr, int *lens, int B,
+                  int min_len, int max_steps, oumu_stream_t stream) {
+    return step_end(false, stop_logits, patch, patches, stop, ctr, lens, B, min_len, max_steps, stream);
+}
+
+int oumu_step_end_live(const void *stop_logits, const void *patch, void *patches, int *stop, int *ctr, int *lens, int B,
+                       int min_len, int max_steps, oumu_stream_t stream) {
+    if (!lens) return OUMU_ERR_INVALID;
+    return step_end(true, stop_logits, patch, patches, stop, ctr, lens, B, min_len, max_steps, stream);
 }
 
 struct oumu_decode_loop_s {

@@ -179,7 +179,9 @@ __global__ void __launch_bounds__(256) k_cfg_euler(bf16 *x, const bf16 *out, int
 
 // End of a decoding step (kernels/voxcpm.cu:415-433), one block: the new patch of every take goes to
 // patches[s][n] (n = ctr[1] < max_steps), a take whose stop logits ask to stop after more than min_len patches
-// records n, then ctr = [position + 1, n + 1] and, with per-take lengths, every lens[s] + 1.
+// records n, then ctr = [position + 1, n + 1] and, with per-take lengths, every lens[s] + 1; LIVE: only of takes that
+// hold positions and had not stopped before this step.
+template <bool LIVE>
 __global__ void __launch_bounds__(256) k_step_end(const bf16 *stop_logits, const bf16 *patch, bf16 *patches,
                                                   int *stop, int *ctr, int *lens, int B, int min_len,
                                                   int max_steps) {
@@ -193,8 +195,9 @@ __global__ void __launch_bounds__(256) k_step_end(const bf16 *stop_logits, const
     }
     for (int s = threadIdx.x; s < B; s += blockDim.x) {
         const bool want = bf2f(stop_logits[2 * s + 1]) > bf2f(stop_logits[2 * s]);
-        if (want && n > min_len && stop[s] < 0) stop[s] = n;
-        if (lens) lens[s] += 1;
+        const bool going = stop[s] < 0;
+        if (want && n > min_len && going) stop[s] = n;
+        if (lens && (!LIVE || (going && lens[s] > 0))) lens[s] += 1;
     }
     __syncthreads();
     if (threadIdx.x == 0) {

@@ -389,8 +389,9 @@ class Engine:
         self.fusion(self.fus, self.res_x)
         self.step_tf(self.res, self.res_x, self.res_h)
         self.cond.copy_(self.x)
+        # on pages, takes that have stopped or were freed get no longer: they would go on taking pages
         ops.step_end(self.stop_l, self.x, self.patches, self.stop, self.ctr, self.lens, B, self.min_len,
-                     self.max_steps)
+                     self.max_steps, live=self.kv4 is not None)
 
     def capture(self, keep_graph=False):
         """The step as one CUDA graph (src/model.rs:779-783), programmatic edges into the decode layers. The step
@@ -416,7 +417,8 @@ class Engine:
     def decode(self, graph, device_loop=True):
         """Steps until every take has stopped or max_steps patches exist; the number of patches of every take
         (Engine::decode, src/model.rs:777-796: stop step + 1, or max_steps for a take that never stopped).
-        device_loop=False replays `graph` and reads the stop flags after every step, as the reference does;
+        device_loop=False replays `graph` and reads the stop flags (and whether pages were missing) after every step, as
+        the reference does;
         device_loop=True runs the whole loop as one graph launch with the stop test on the device (`graph` from
         capture(keep_graph=True)) and reads the flags once."""
         if device_loop:
@@ -437,5 +439,6 @@ class Engine:
                     break
                 graph.replay()
                 stops = self.stop.cpu()
+                self._check_pages()
         self._check_pages()
         return [int(v) + 1 if v >= 0 else self.max_steps for v in stops.tolist()]

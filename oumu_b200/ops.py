@@ -195,8 +195,9 @@ def cfg_euler(x, out, B, seq, first, dt, cfg):
     return x
 
 
-def step_end(stop_logits, patch, patches, stop, ctr, lens, B, min_len, max_steps):
-    _lib.call("oumu_step_end", _p(stop_logits), _p(patch), _p(patches), _p(stop), _p(ctr), _p(lens), B, min_len,
+def step_end(stop_logits, patch, patches, stop, ctr, lens, B, min_len, max_steps, live=False):
+    """live: only takes that hold positions and had not stopped get longer (oumu_step_end_live)."""
+    _lib.call("oumu_step_end_live" if live else "oumu_step_end", _p(stop_logits), _p(patch), _p(patches), _p(stop), _p(ctr), _p(lens), B, min_len,
               max_steps, _stream())
 
 
