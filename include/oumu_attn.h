@@ -272,7 +272,8 @@ int oumu_attn_decode_kv4_step(const void *qkv, void *pool, void *out, void *held
 /*
  * Pages of a cache, for any contents: the pool of layer l is `pools` + l * layer_stride, npages pages of page_bytes
  * (both multiples of 16). They read and change tables on the device, in an order that does not depend on timing, and
- * can be captured; launches on one table and ref must be ordered with each other.
+ * can be captured; launches on one table and ref must be ordered with each other. Every call writes its status anew: a
+ * fork and an extend whose statuses are read later have one each (the extend lacks nothing for takes the fork left empty).
  *
  * extend: every take with lens[s] > 0 gets the pages it lacks for its first lens[s] + extra positions (a step appends
  * with extra 0 once lens counts the newest position): free pages, lowest first, in the order of takes and positions.

@@ -269,6 +269,7 @@ class Engine:
         """Pages with random K/V: the prompt in take 0, forked to the others, then every take's own positions."""
         c, B, dev = self.kv4, self.B, self.device
         c.free(range(B))
+        c.status.zero_()  # what earlier takes lacked
         self._prompt = prompt
         if prompt:
             row = torch.empty((prompt, 2 * NK * HD), dtype=torch.bfloat16, device=dev)
@@ -288,9 +289,9 @@ class Engine:
         self._check_pages()
 
     def _check_pages(self):
-        if self.kv4 is not None and int(self.kv4.status[0]):
-            raise RuntimeError(f"the 4-bit cache's {self.kv4.npages} pages do not hold the takes: "
-                               f"{int(self.kv4.status[0])} pages are missing")
+        short = self.kv4.missing() if self.kv4 is not None else 0
+        if short:
+            raise RuntimeError(f"the 4-bit cache's {self.kv4.npages} pages do not hold the takes: {short} pages are missing")
 
     def set_lens(self, lens):
         if self.kv4 is not None and min(int(v) for v in lens) <= getattr(self, "_prompt", 0):

@@ -25,7 +25,9 @@ class KV4Cache:
         self.pools = torch.empty((layers, npages, ops.kv4_page_bytes(nk, hd)), dtype=torch.uint8, device=dev)
         self.table = torch.full((B, self.maxpages), -1, dtype=torch.int32, device=dev)
         self.ref, self.lens = i32(npages), i32(B) if lens is None else lens
-        self.status, self.moved = i32(2), i32(2)  # [pages missing], [pages in use, pages moved]
+        # pages missing: [what extends lacked at most, what forks lacked in all] since `missing` was last asked, and of the
+        # last call of each; [pages in use, pages moved]
+        self.status, self._last, self.moved = i32(2), i32(2), i32(2)
         self.ws = ops.decode_kv4_workspace(B, nq, nk, hd, self.maxpages, dev)
         self._pages_ws = ops.pages_workspace(npages, dev)
 
@@ -33,12 +35,24 @@ class KV4Cache:
         return torch.as_tensor(takes, dtype=torch.int32).to(self.table.device)
 
     def extend(self, extra=0):
-        """Pages for every take's first lens + extra positions; status[0] counts those the pool did not have."""
-        ops.pages_extend(self.table, self.ref, self.lens, extra, self.status)
+        """Pages for every take's first lens + extra positions. Those that the pool did not have are missing until
+        `missing` is asked, whatever later calls find: what was to be written there is lost."""
+        ops.pages_extend(self.table, self.ref, self.lens, extra, self._last[:1])
+        torch.maximum(self.status[:1], self._last[:1], out=self.status[:1])
 
     def fork(self, src, dst):
-        """Takes dst[i] continue where takes src[i] are, on shared pages (device int32 tensors, or lists)."""
-        ops.pages_fork(self.pools, self.table, self.ref, self.lens, self._ids(src), self._ids(dst), self.status)
+        """Takes dst[i] continue where takes src[i] are, on shared pages (device int32 tensors, or lists). Takes for which
+        no page was left end up empty; `missing` counts them."""
+        ops.pages_fork(self.pools, self.table, self.ref, self.lens, self._ids(src), self._ids(dst), self._last[1:])
+        self.status[1:].add_(self._last[1:])
+
+    def missing(self):
+        """Pages that extends (the most any one lacked) and forks (each) did not get since the last time this was asked;
+        waits for the GPU."""
+        n = sum(self.status.tolist())
+        if n:
+            self.status.zero_()
+        return n
 
     def free(self, takes):
         ops.pages_free(self.table, self.ref, self.lens, self._ids(takes))
