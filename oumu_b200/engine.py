@@ -202,6 +202,7 @@ class Engine:
             pages = B * -(-maxlen // ops.KV4_PAGE) if kv_pages is None else kv_pages
             self.kv4 = KV4Cache(base_layers + res_layers, B, NQ, NK, HD, pages, maxlen, dev, lens=self.lens)
         self._scratch = {}
+        self._prompt = 0
 
     def _temb(self, ini):
         """Time embedding of every DiT pass, time_mlp(sinusoid(t)) + delta_time_mlp(sinusoid(0))
@@ -294,9 +295,19 @@ class Engine:
             raise RuntimeError(f"the 4-bit cache's {self.kv4.npages} pages do not hold the takes: {short} pages are missing")
 
     def set_lens(self, lens):
-        if self.kv4 is not None and min(int(v) for v in lens) <= getattr(self, "_prompt", 0):
-            raise ValueError("a take's newest position lies behind the prompt it shares")
-        self.lens.copy_(torch.as_tensor([int(v) for v in lens], dtype=torch.int32))
+        """lens[s]: positions take s attends over in the next step, its newest one written by it. On pages, at most as many
+        as it has now (behind them its pages hold nothing, where bf16 slots are primed to their ends), and 0 for a take that
+        was freed, which stays so."""
+        lens = [int(v) for v in lens]
+        if self.kv4 is not None:
+            rows, ref = self.kv4.table.tolist(), self.kv4.ref.tolist()
+            for n, now, row in zip(lens, self.lens.tolist(), rows, strict=True):
+                if n > now:
+                    raise ValueError(f"a take of {now} positions cannot go on from {n}")
+                page = row[(n - 1) // ops.KV4_PAGE] if n > 0 else -1
+                if (n <= self._prompt and (n or now)) or (page >= 0 and ref[page] > 1):
+                    raise ValueError("a take's newest position lies among those it shares")
+        self.lens.copy_(torch.as_tensor(lens, dtype=torch.int32))
         self.ctr.zero_()
         self.stop.fill_(-1)
 

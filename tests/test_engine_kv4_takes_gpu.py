@@ -1,4 +1,4 @@
-"""Takes of Engine(kv="int4") that stop or are freed while others go on."""
+"""Takes of Engine(kv="int4") that stop or are freed while others go on, or are given lengths they do not hold."""
 import pytest
 import torch
 
@@ -67,6 +67,46 @@ def test_a_freed_take_stays_free(cuda):
     assert e.lens.tolist() == [69, 0, 84]
     assert e.kv4.table[1].max().item() == -1 and int((e.kv4.ref > 0).sum()) == used - 2
     assert ops.device_error() == 0
+    # decode on: the other takes from where they are
+    e.set_lens([60, 0, 80])
+    e.step()
+    torch.cuda.synchronize()
+    assert e.lens.tolist() == [61, 0, 81] and ops.device_error() == 0
+
+
+def test_set_lens_refuses_positions_that_no_take_holds(cuda):
+    e = make(2)
+    e.prime([70, 100])
+    with pytest.raises(ValueError):
+        e.set_lens([71, 100])  # position 70 would be read as the page was left
+    with pytest.raises(ValueError):
+        e.set_lens([70, 300])
+    with pytest.raises(ValueError):
+        e.set_lens([0, 100])
+    e.set_lens([70, 100])
+    e.step()
+    torch.cuda.synchronize()
+    assert e.lens.tolist() == [71, 101]
+    e.set_lens([71, 90])
+    e.step()
+    torch.cuda.synchronize()
+    assert e.lens.tolist() == [72, 91] and ops.device_error() == 0
+    b = make(2, kv="bf16")
+    b.prime([70, 100])
+    b.set_lens([200, 300])  # bf16 slots are filled to their ends
+
+
+def test_set_lens_refuses_positions_that_takes_share(cuda):
+    e = make(2)
+    e.prime([130, 70])
+    e.kv4.fork([0], [1])  # positions 0..127 on shared pages
+    with pytest.raises(ValueError):
+        e.set_lens([100, 130])
+    with pytest.raises(ValueError):
+        e.set_lens([130, 128])
+    e.set_lens([129, 130])
+    with pytest.raises(ValueError):
+        e.set_lens([129])
 
 
 def test_a_pool_that_runs_out_is_noticed_at_once(cuda):
