@@ -12,8 +12,11 @@
 // so the matrix instructions multiply by the codes themselves: fp16 subnormals n 2^-24, exact, masked out of the
 // packed words. q is scaled by a power of two of its own for each head so that it is exact in fp16; the zeros' term of
 // the scores is one more instruction, bf16 zeros times Q split into three bf16 parts (24 bits). p_j s_jg is rounded to
-// fp16 (2^-12 relative): its running reference M keeps the largest near 2^10, far from fp16's limits at both ends,
-// and moves only when a product passes 2^15. Sums, p, the zeros' term of the output and M are fp32.
+// fp16 (2^-11 relative, at most): a power of two of each group's own brings the group's largest scale to [2^9, 2^10), and
+// the head's running reference M the largest product to about 2^10, so V may be of any size, and one group's size costs
+// another nothing. Both move only when a product passes 2^15 (or p does, so that no sum of p z of 65536 positions and
+// |z| up to 2^95 leaves fp32). A scale keeps all bits of p s down to 2^-24 of its group's largest. Sums, p, the zeros'
+// term of the output and M are fp32.
 // The tensor cores cut their sums off instead of rounding them, a bias that grows with the number of positions while
 // the result, an average of values of either sign, shrinks: codes 0..15 of one sign left 6e-3 relative error at 65536
 // positions. So an odd position's value is taken as s (n - 15) + (z + 15 s): the codes of even and odd positions then
@@ -29,7 +32,7 @@ using kv4::HALF;
 using kv4::Words;
 
 constexpr int GMAX = 8;      // q heads per kv head handled by one mma column block
-constexpr float SMIN = 8.6736174e-19f;  // 2^-60: groups of smaller scale count as this when M is set
+constexpr uint32_t GAIN_MAX = 0x7e807e80u;  // a pair of 2^126: for groups whose scales have all been 0 (and subnormal ones)
 
 // Not volatile (nor the transposition below): the compiler may interleave these with other work as it likes.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -86,6 +89,14 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
+}
+__device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    return kv4::as_u32(__hmul2(kv4::as_bf2(a), kv4::as_bf2(b)));
 }
 
 struct Params {
@@ -206,12 +217,15 @@ struct State {
     static constexpr int W = Fmt<HD>::W;
     static constexpr bool SIDE = W == 4;
     float M[2];                // reference exponent
-    float acc[2 * W][4];       // numerator / 2^24 of channels 32w + 4g + {0 | 1 (x 16)}, {2 | 3 (x 16)}
+    uint32_t gain[W / 2];      // the groups' powers of two, as bf16 pairs like a meta row's scales
+    float acc[2 * W][4];       // numerator * gain / 2^24 of channels 32w + 4g + {0 | 1 (x 16)}, {2 | 3 (x 16)}
     // SIDE: [0..1] row g: sum p s_g (g < 4, not used) | sum p z of group g - 4; [2..3] row 8 + g: sum over odd positions
     // of p s_g (g < 4) | sum p. Otherwise: [2w + c] this lane's share of the zeros' term, [2W + c] of the sum.
     float side[SIDE ? 4 : 2 * W + 2];
     __device__ void clear() {
         M[0] = M[1] = -INFINITY;
+#pragma unroll
+        for (uint32_t &f : gain) f = GAIN_MAX;
 #pragma unroll
         for (int i = 0; i < 2 * W; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
@@ -287,16 +301,20 @@ struct State {
                 for (int i = 0; i < 4; i++) p[h][i] = fast_exp2(fmaf(x[h][i], i & 1 ? Q.mul1 : Q.mul0, -M[i & 1]));
                 big = fmax3(fmax3(big, p[h][0], p[h][1]), p[h][2], p[h][3]);
 #pragma unroll
-                for (int w = 0; w < W; w++)
+                for (int r = 0; r < 2; r++) {
+                    Words<W> sg;
 #pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        const float s = kv4::row_scale<W>(vm[h][r], w);
+                    for (int i = 0; i < W / 2; i++) sg.v[i] = mul_bf16x2(vm[h][r].v[i], gain[i]);  // exact
+#pragma unroll
+                    for (int w = 0; w < W; w++) {
+                        const float s = kv4::row_scale<W>(sg, w);
                         pv[h][w][r] = pack_f16x2(p[h][2 * r] * s, p[h][2 * r + 1] * s);
                         top = max_u16x2(top, pv[h][w][r]);
                     }
+                }
             }
-            // 2^15 in fp16 is 0x7800 (infinities and NaN lie above); p itself may reach 2^75 where every scale is tiny
-            const bool over = (top & 0xffffu) > 0x7800u || top > 0x7800ffffu || !(big <= 3.7778932e22f);
+            // 2^15 in fp16 is 0x7800 (infinities and NaN lie above)
+            const bool over = (top & 0xffffu) > 0x7800u || top > 0x7800ffffu || !(big <= 32768.f);
             if (again || !__any_sync(0xffffffffu, over)) break;
             rescale(x, vm, Q);
         }
@@ -349,18 +367,28 @@ struct State {
         }
     }
 
-    // Raise M so that the largest p s of this tile is 2^10, and bring the sums along. The first tile of a state always
-    // comes here (M = -inf); later ones when a logit rises by more than 5 over everything before.
+    // Lower the gains so that no scale of this tile passes 2^10, raise M so that the largest p s is 2^10 (or p, where the
+    // scales that count are below 1), and bring the sums along. The first tile of a state always comes here (M = -inf);
+    // later ones when a logit, or a scale, rises by more than 2^5 over everything before.
     __device__ __forceinline__ void rescale(const float (&x)[2][4], const Words<W> (&vm)[2][2], const Query<HD> &Q) {
+        uint32_t now[W / 2];
+#pragma unroll
+        for (int i = 0; i < W / 2; i++) {
+            const uint32_t m = max_u16x2(max_u16x2(vm[0][0].v[i], vm[0][1].v[i]), max_u16x2(vm[1][0].v[i], vm[1][1].v[i]));
+            const uint32_t lo = __reduce_max_sync(0xffffffffu, m << 16), hi = __reduce_max_sync(0xffffffffu, m);
+            // exponent fields: 2^(9 - e) for a scale in [2^e, 2^(e + 1)), e + 127 being the scale's own (0: GAIN_MAX)
+            now[i] = min_u16x2(gain[i], 0x83808380u - (__byte_perm(lo, hi, 0x7632) & 0x7f807f80u));
+        }
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                float s = SMIN;
+                uint32_t sg = 0x3f803f80u;  // a pair of 1
 #pragma unroll
-                for (int w = 0; w < W; w++) s = fmaxf(s, kv4::row_scale<W>(vm[h][r], w));
-                const float ls = __log2f(s);
+                for (int i = 0; i < W / 2; i++)  // (a NaN is passed over)
+                    sg = kv4::as_u32(__hmax2(kv4::as_bf2(sg), kv4::as_bf2(mul_bf16x2(vm[h][r].v[i], now[i]))));
+                const float ls = __log2f(fmaxf(__uint_as_float(sg << 16), __uint_as_float(sg & 0xffff0000u)));
                 top[0] = fmaxf(top[0], fmaf(x[h][2 * r], Q.mul0, ls));
                 top[1] = fmaxf(top[1], fmaf(x[h][2 * r + 1], Q.mul1, ls));
             }
@@ -368,18 +396,33 @@ struct State {
         for (int c = 0; c < 2; c++) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-            float m = fmaxf(M[c], top[c] - 10.f);
-            if (m == -INFINITY) m = 0.f;
-            const float f = fast_exp2(M[c] - m);
-            M[c] = m;
-#pragma unroll
-            for (int i = 0; i < 2 * W; i++) {
-                acc[i][c] *= f;
-                acc[i][c + 2] *= f;
-            }
-#pragma unroll
-            for (int i = c; i < (SIDE ? 4 : 2 * W + 2); i += 2) side[i] *= f;
+            top[c] = fmaxf(M[c], top[c] - 10.f);
+            if (top[c] == -INFINITY) top[c] = 0.f;
         }
+        if (M[0] != -INFINITY) {  // some sums there are
+            float g[W];  // now / gain, 0 below 2^-149
+#pragma unroll
+            for (int w = 0; w < W; w++) g[w] = pick(now, w) * __uint_as_float(0x7f000000u - __float_as_uint(pick(gain, w)));
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const float f = fast_exp2(M[c] - top[c]);
+#pragma unroll
+                for (int i = 0; i < 2 * W; i++) {
+                    acc[i][c] *= f * g[i / 2];
+                    acc[i][c + 2] *= f * g[i / 2];
+                }
+#pragma unroll
+                for (int i = c; i < (SIDE ? 4 : 2 * W + 2); i += 2) side[i] *= f;
+            }
+        }
+        M[0] = top[0];
+        M[1] = top[1];
+#pragma unroll
+        for (int i = 0; i < W / 2; i++) gain[i] = now[i];
+    }
+    // Group w's of pairs of bf16
+    __device__ __forceinline__ static float pick(const uint32_t (&v)[W / 2], int w) {
+        return __uint_as_float(w & 1 ? v[w / 2] & 0xffff0000u : v[w / 2] << 16);
     }
 
     // The sums of p and the zeros' terms of heads 2t and 2t + 1 over all positions, in every lane.
@@ -409,8 +452,9 @@ struct State {
     // Numerators of head 2t + c, channels 32w + 4g .. + 3, with the zeros' term, in the values' own unit.
     __device__ __forceinline__ float4 numerators(const float (&z)[W][2], int w, int c) const {
         const float u = 16777216.f, u16 = 1048576.f;  // 2^24, and / 16 for the odd nibbles
-        return make_float4(fmaf(acc[2 * w][c], u, z[w][c]), fmaf(acc[2 * w][c + 2], u16, z[w][c]),
-                           fmaf(acc[2 * w + 1][c], u, z[w][c]), fmaf(acc[2 * w + 1][c + 2], u16, z[w][c]));
+        const float r = __uint_as_float(0x7f000000u - __float_as_uint(pick(gain, w)));  // 1 / gain
+        return make_float4(fmaf(acc[2 * w][c] * u, r, z[w][c]), fmaf(acc[2 * w][c + 2] * u16, r, z[w][c]),
+                           fmaf(acc[2 * w + 1][c] * u, r, z[w][c]), fmaf(acc[2 * w + 1][c + 2] * u16, r, z[w][c]));
     }
     // The output of a segment that this warp has seen whole; out: its first head's row.
     __device__ __forceinline__ void finish(bf16 *out, int G, int lane) {

@@ -1,10 +1,11 @@
-"""The 4-bit paged cache at its limits: lengths that its tables do not hold, pools that run out."""
+"""The 4-bit paged cache at its limits: lengths that its tables do not hold, V of any size a bf16
+has, pools that run out."""
 import pytest
 import torch
 
 from oumu_b200 import ops
 from oumu_b200.kv4 import KV4Cache
-from test_kv4_gpu import LENGTH, attn_case, i32, randn, run_attn
+from test_kv4_gpu import LENGTH, attn_case, check_attn, i32, randn, run_attn
 
 pytestmark = pytest.mark.gpu
 
@@ -30,6 +31,76 @@ def test_a_step_past_the_end_writes_nothing(cuda, what, hd):
     assert ops.device_error(reset=True) == LENGTH
     assert torch.equal(pool, before)
     assert torch.equal(run_attn(qkv, pool, table, i32([128] * B), B, nq, nk, hd), want)
+
+
+# ---- V of any size ----
+
+def sized(kind, T, nk, hd, dev="cuda"):
+    """T rows of k and v [T][2][nk][hd]."""
+    kv = randn(95, T, 2 * nk * hd).float().view(T, 2, nk, hd)
+    v = kv[:, 1]
+    part, _, arg = kind.partition(":")
+    x = float(arg) if arg else 0.0
+    if part == "all":
+        v *= x
+    elif part == "group":            # one group of every position
+        v[..., 32:64] *= x
+    elif part == "constant":
+        v[:] = x
+    elif part == "constant_and":     # a constant group beside one of another size
+        v[..., :32] = 1e20
+        v[..., 32:64] *= x
+    elif part == "late":             # a group that is 0 at first
+        v[..., 32:64] *= x
+        v[:T // 2, :, 32:64] = 0
+    elif part == "growing":          # from 1e-20 to 1e10 along the positions
+        v *= 10.0 ** torch.linspace(-20, 10, T, device=dev).view(T, 1, 1)
+    elif part == "falling":
+        v *= 10.0 ** torch.linspace(10, -20, T, device=dev).view(T, 1, 1)
+    elif part == "some":             # one position in 50 is larger in one group
+        v[::50, :, 32:64] *= x
+    return kv.bfloat16().view(T, -1)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", ["all:1e-25", "all:1e-28", "all:1e-32", "all:1e-35", "all:1e30", "group:1e-9",
+                                  "group:1e-12", "group:1e-25", "group:1e12", "group:1e25", "constant:1e20",
+                                  "constant:-1e30", "constant:1e-30", "constant_and:1e-9", "constant_and:1e9",
+                                  "late:1e-15", "late:1e15", "growing", "falling", "some:1e6", "some:1e-12"])
+def test_attention_with_v_of_any_size(cuda, kind, hd):
+    """The bound of check_attn, each channel's own: what one group holds costs another nothing."""
+    nq, nk, lens = 8, 2, [500, 97]
+    kv = torch.cat([sized(kind, 500, nk, hd), sized(kind, 500, nk, hd).flip(0)])
+    qkv, pool, rows, table, ln = attn_case(lens, nq, nk, hd, seed=96, kv=kv)
+    check_attn(run_attn(qkv, pool, table, ln, 2, nq, nk, hd), qkv, pool, rows, lens, nq, nk, hd)
+
+
+@pytest.mark.parametrize("kind", ["group:1e-12", "all:1e-30", "constant_and:1e-9", "growing", "falling"])
+def test_split_attention_with_v_of_any_size(cuda, kind):
+    nq, nk, hd, lens = 16, 2, 128, [20000]
+    qkv, pool, rows, table, ln = attn_case(lens, nq, nk, hd, seed=97, kv=sized(kind, 20000, nk, hd))
+    check_attn(run_attn(qkv, pool, table, ln, 1, nq, nk, hd), qkv, pool, rows, lens, nq, nk, hd)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group", [0, 1])
+def test_nan_in_a_group_of_v_stays_in_it(cuda, hd, group):
+    nq, nk, n = 4, 2, 300
+    kv = randn(101, n, 2 * nk * hd).view(n, 2, nk, hd)
+    bad = kv.clone()
+    bad[[0, 5, 250], 1, 1, 32 * group + 7] = float("nan")
+    good, out = [], []
+    for x, to in ((kv, good), (bad, out)):
+        qkv, pool, rows, table, ln = attn_case([n], nq, nk, hd, seed=102, kv=x.view(n, -1))
+        to.append(run_attn(qkv, pool, table, ln, 1, nq, nk, hd).view(nq, hd).float())
+    good, out = good[0], out[0]
+    hit = torch.zeros(nq, hd, dtype=torch.bool, device="cuda")
+    hit[2:, 32 * group:32 * group + 32] = True
+    assert bool(torch.isnan(out[hit]).all()) and not bool(torch.isnan(out[~hit]).any())
+    # the bound of check_attn, of both, with 15 s <= the spread (1 + 2^-7), which is at most twice the largest |V|
+    big = float(kv[:, 1].abs().max())
+    tol = 2 * (good.abs() * 2 ** -8 + 2 * big * (1 + 2 ** -7) * (2 ** -11 + 2 ** -14) + big * 2 ** -14)
+    assert bool(((out - good).abs() <= tol)[~hit].all())
 
 
 # ---- the cache's own calls ----
