@@ -14,9 +14,9 @@
 // the scores is one more instruction, bf16 zeros times Q split into three bf16 parts (24 bits). p_j s_jg is rounded to
 // fp16 (2^-11 relative, at most): a power of two of each group's own brings the group's largest scale to [2^9, 2^10), and
 // the head's running reference M the largest product to about 2^10, so V may be of any size, and one group's size costs
-// another nothing. Both move only when a product passes 2^15 (or p does, so that no sum of p z of 65536 positions and
-// |z| up to 2^95 leaves fp32). A scale keeps all bits of p s down to 2^-24 of its group's largest. Sums, p, the zeros'
-// term of the output and M are fp32.
+// another nothing. Both move only when a product passes 2^15 (or p does: with |z| up to 2^95 no sum of p z of 65536
+// positions leaves fp32; larger z lift M, and the powers with it). A scale keeps all bits of p s down to 2^-24 of its
+// group's largest. Sums, p, the zeros' term of the output and M are fp32.
 // The tensor cores cut their sums off instead of rounding them, a bias that grows with the number of positions while
 // the result, an average of values of either sign, shrinks: codes 0..15 of one sign left 6e-3 relative error at 65536
 // positions. So an odd position's value is taken as s (n - 15) + (z + 15 s): the codes of even and odd positions then
@@ -218,6 +218,7 @@ struct State {
     static constexpr bool SIDE = W == 4;
     float M[2];                // reference exponent
     uint32_t gain[W / 2];      // the groups' powers of two, as bf16 pairs like a meta row's scales
+    int lift;                  // how far M and the gains are raised for large z, in factors of 2
     float acc[2 * W][4];       // numerator * gain / 2^24 of channels 32w + 4g + {0 | 1 (x 16)}, {2 | 3 (x 16)}
     // SIDE: [0..1] row g: sum p s_g (g < 4, not used) | sum p z of group g - 4; [2..3] row 8 + g: sum over odd positions
     // of p s_g (g < 4) | sum p. Otherwise: [2w + c] this lane's share of the zeros' term, [2W + c] of the sum.
@@ -226,6 +227,7 @@ struct State {
         M[0] = M[1] = -INFINITY;
 #pragma unroll
         for (uint32_t &f : gain) f = GAIN_MAX;
+        lift = 0;
 #pragma unroll
         for (int i = 0; i < 2 * W; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
@@ -368,23 +370,33 @@ struct State {
     }
 
     // Lower the gains so that no scale of this tile passes 2^10, raise M so that the largest p s is 2^10 (or p, where the
-    // scales that count are below 1), and bring the sums along. The first tile of a state always comes here (M = -inf);
+    // scales that count are below 1), both times 2^lift and 2^-lift, and bring the sums along. The first tile of a state always comes here (M = -inf);
     // later ones when a logit, or a scale, rises by more than 2^5 over everything before.
     __device__ __forceinline__ void rescale(const float (&x)[2][4], const Words<W> (&vm)[2][2], const Query<HD> &Q) {
-        uint32_t now[W / 2];
+        uint32_t now[W / 2], zmax = 0;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int i = 0; i < W / 2; i++) zmax = max_u16x2(zmax, vm[h][r].v[W / 2 + i] & 0x7fff7fffu);
+        zmax = __reduce_max_sync(0xffffffffu, max(zmax << 16, zmax));
+        const int more = max(static_cast<int>(zmax >> 23) - (127 + 95) - lift, 0);  // |z| from 2^95 on
+        lift += more;
 #pragma unroll
         for (int i = 0; i < W / 2; i++) {
             const uint32_t m = max_u16x2(max_u16x2(vm[0][0].v[i], vm[0][1].v[i]), max_u16x2(vm[1][0].v[i], vm[1][1].v[i]));
             const uint32_t lo = __reduce_max_sync(0xffffffffu, m << 16), hi = __reduce_max_sync(0xffffffffu, m);
-            // exponent fields: 2^(9 - e) for a scale in [2^e, 2^(e + 1)), e + 127 being the scale's own (0: GAIN_MAX)
-            now[i] = min_u16x2(gain[i], 0x83808380u - (__byte_perm(lo, hi, 0x7632) & 0x7f807f80u));
+            // exponent fields: 2^(9 + lift - e) for a scale in [2^e, 2^(e + 1)), e + 127 being the scale's own (0: GAIN_MAX)
+            const uint32_t want = 0x83808380u + lift * 0x800080u - (__byte_perm(lo, hi, 0x7632) & 0x7f807f80u);
+            now[i] = min_u16x2(min_u16x2(gain[i] + more * 0x800080u, GAIN_MAX), want);
         }
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                uint32_t sg = 0x3f803f80u;  // a pair of 1
+                uint32_t sg = 0x3f803f80u + lift * 0x800080u;  // a pair of 2^lift
 #pragma unroll
                 for (int i = 0; i < W / 2; i++)  // (a NaN is passed over)
                     sg = kv4::as_u32(__hmax2(kv4::as_bf2(sg), kv4::as_bf2(mul_bf16x2(vm[h][r].v[i], now[i]))));
@@ -396,7 +408,7 @@ struct State {
         for (int c = 0; c < 2; c++) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-            top[c] = fmaxf(M[c], top[c] - 10.f);
+            top[c] = fmaxf(M[c] + more, top[c] - 10.f);
             if (top[c] == -INFINITY) top[c] = 0.f;
         }
         if (M[0] != -INFINITY) {  // some sums there are

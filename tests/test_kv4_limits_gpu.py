@@ -63,10 +63,13 @@ def sized(kind, T, nk, hd, dev="cuda"):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("kind", ["all:1e-25", "all:1e-28", "all:1e-32", "all:1e-35", "all:1e30", "group:1e-9",
-                                  "group:1e-12", "group:1e-25", "group:1e12", "group:1e25", "constant:1e20",
-                                  "constant:-1e30", "constant:1e-30", "constant_and:1e-9", "constant_and:1e9",
-                                  "late:1e-15", "late:1e15", "growing", "falling", "some:1e6", "some:1e-12"])
+KINDS = ["all:1e-25", "all:1e-28", "all:1e-32", "all:1e-35", "all:1e30", "all:1e33", "all:3e37", "group:1e-9", "group:1e-12",
+         "group:1e-25", "group:1e12", "group:1e25", "constant:1e20", "constant:-1e30", "constant:-3e38", "constant:1e-30",
+         "constant_and:1e-9", "constant_and:1e9", "late:1e-15", "late:1e15", "growing", "falling", "some:1e6", "some:1e-12"]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", KINDS)
 def test_attention_with_v_of_any_size(cuda, kind, hd):
     """The bound of check_attn, each channel's own: what one group holds costs another nothing."""
     nq, nk, lens = 8, 2, [500, 97]
@@ -75,7 +78,8 @@ def test_attention_with_v_of_any_size(cuda, kind, hd):
     check_attn(run_attn(qkv, pool, table, ln, 2, nq, nk, hd), qkv, pool, rows, lens, nq, nk, hd)
 
 
-@pytest.mark.parametrize("kind", ["group:1e-12", "all:1e-30", "constant_and:1e-9", "growing", "falling"])
+@pytest.mark.parametrize("kind", ["group:1e-12", "all:1e-30", "all:3e37", "constant_and:1e-9", "constant:3e38", "growing",
+                                  "falling"])
 def test_split_attention_with_v_of_any_size(cuda, kind):
     nq, nk, hd, lens = 16, 2, 128, [20000]
     qkv, pool, rows, table, ln = attn_case(lens, nq, nk, hd, seed=97, kv=sized(kind, 20000, nk, hd))
