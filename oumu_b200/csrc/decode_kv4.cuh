@@ -12,11 +12,11 @@
 // so the matrix instructions multiply by the codes themselves: fp16 subnormals n 2^-24, exact, masked out of the
 // packed words. q is scaled by a power of two of its own for each head so that it is exact in fp16; the zeros' term of
 // the scores is one more instruction, bf16 zeros times Q split into three bf16 parts (24 bits). p_j s_jg is rounded to
-// fp16 (2^-11 relative, at most): a power of two of each group's own brings the group's largest scale to [2^9, 2^10), and
-// the head's running reference M the largest product to about 2^10, so V may be of any size, and one group's size costs
-// another nothing. Both move only when a product passes 2^15 (or p does: with |z| up to 2^95 no sum of p z of 65536
-// positions leaves fp32; larger z lift M, and the powers with it). A scale keeps all bits of p s down to 2^-24 of its
-// group's largest. Sums, p, the zeros' term of the output and M are fp32.
+// fp16 (2^-11 relative, at most). The head's running reference M, a raw score, keeps the largest p at 2^-12: no sum of p z
+// leaves fp32, and M is exact however large the scores are. A power of two of each channel group's own, its gain, keeps the
+// group's largest scale at 2^21 or more: the largest products are near 2^9, V may be of any size, and one group's size
+// costs another nothing. Both move only when p or a product rises by more than 2^5. A scale keeps all bits of p s down to
+// 2^-23 of its group's largest. Sums, p, the zeros' term of the output and M are fp32.
 // The tensor cores cut their sums off instead of rounding them, a bias that grows with the number of positions while
 // the result, an average of values of either sign, shrinks: codes 0..15 of one sign left 6e-3 relative error at 65536
 // positions. So an odd position's value is taken as s (n - 15) + (z + 15 s): the codes of even and odd positions then
@@ -161,9 +161,9 @@ struct Query {
             for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[w][i]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // the largest |q| of the head lands in [2^14, 2^15): fp16 keeps a bf16 exactly down to 2^-28 of it
-        int e = 14 - (static_cast<int>(__float_as_uint(mx) >> 23) - 127);
-        e = e > 100 ? 100 : e < -90 ? -90 : e;
+        // the largest |q| of the head lands in [2^14, 2^15): fp16 keeps a bf16 exactly down to 2^-27 of it
+        int e = mx > 0.f ? 14 + 127 - static_cast<int>(__float_as_uint(mx) >> 23) : 14;
+        e = e > 127 ? 127 : e;
         const float f = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
         float sum[W];
 #pragma unroll
@@ -202,7 +202,11 @@ struct Query {
             z0 = t == 0 ? part[0][0] : t == 1 ? part[1][0] : t == 2 ? part[2][0] : 0u;
             z1 = 0u;
         }
-        const float m = __uint_as_float(static_cast<uint32_t>(24 - e + 127) << 23) * P.sl2;
+        // 2^(24 - e), by the units of q and of the codes, in two factors. Kept inside fp32, where products with 0 and infinity
+        // have a value (the upper end is met where |q| scale reaches 2^117)
+        float m = __uint_as_float(static_cast<uint32_t>((24 - e) / 2 + 127) << 23);
+        m = m * P.sl2 * m * (e & 1 ? e < 24 ? 2.f : 0.5f : 1.f);
+        m = fminf(fmaxf(m, 1.17549435e-38f), 3.40282347e38f);
         mul0 = __shfl_sync(0xffffffffu, m, 8 * t);
         mul1 = __shfl_sync(0xffffffffu, m, 8 * t + 4);
     }
@@ -216,9 +220,8 @@ template <int HD>
 struct State {
     static constexpr int W = Fmt<HD>::W;
     static constexpr bool SIDE = W == 4;
-    float M[2];                // reference exponent
+    float M[2];                // the reference: the largest raw score, or a little less
     uint32_t gain[W / 2];      // the groups' powers of two, as bf16 pairs like a meta row's scales
-    int lift;                  // how far M and the gains are raised for large z, in factors of 2
     float acc[2 * W][4];       // numerator * gain / 2^24 of channels 32w + 4g + {0 | 1 (x 16)}, {2 | 3 (x 16)}
     // SIDE: [0..1] row g: sum p s_g (g < 4, not used) | sum p z of group g - 4; [2..3] row 8 + g: sum over odd positions
     // of p s_g (g < 4) | sum p. Otherwise: [2w + c] this lane's share of the zeros' term, [2W + c] of the sum.
@@ -227,7 +230,6 @@ struct State {
         M[0] = M[1] = -INFINITY;
 #pragma unroll
         for (uint32_t &f : gain) f = GAIN_MAX;
-        lift = 0;
 #pragma unroll
         for (int i = 0; i < 2 * W; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
@@ -300,7 +302,7 @@ struct State {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) p[h][i] = fast_exp2(fmaf(x[h][i], i & 1 ? Q.mul1 : Q.mul0, -M[i & 1]));
+                for (int i = 0; i < 4; i++) p[h][i] = fast_exp2(fmaf(x[h][i] - M[i & 1], i & 1 ? Q.mul1 : Q.mul0, -12.f));
                 big = fmax3(fmax3(big, p[h][0], p[h][1]), p[h][2], p[h][3]);
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
@@ -315,8 +317,8 @@ struct State {
                     }
                 }
             }
-            // 2^15 in fp16 is 0x7800 (infinities and NaN lie above)
-            const bool over = (top & 0xffffu) > 0x7800u || top > 0x7800ffffu || !(big <= 32768.f);
+            // 2^-7, and 2^15 in fp16 (0x7800; infinities and NaN lie above)
+            const bool over = (top & 0xffffu) > 0x7800u || top > 0x7800ffffu || !(big <= 0.0078125f);
             if (again || !__any_sync(0xffffffffu, over)) break;
             rescale(x, vm, Q);
         }
@@ -369,47 +371,26 @@ struct State {
         }
     }
 
-    // Lower the gains so that no scale of this tile passes 2^10, raise M so that the largest p s is 2^10 (or p, where the
-    // scales that count are below 1), both times 2^lift and 2^-lift, and bring the sums along. The first tile of a state always comes here (M = -inf);
-    // later ones when a logit, or a scale, rises by more than 2^5 over everything before.
+    // Raise M to the largest score of this tile, lower the gains so that no scale passes 2^22, and bring the sums along. The
+    // first tile of a state always comes here (M = -inf); later ones when a logit rises by more than 5 over everything
+    // before, or a scale by more than 2^5.
     __device__ __forceinline__ void rescale(const float (&x)[2][4], const Words<W> (&vm)[2][2], const Query<HD> &Q) {
-        uint32_t now[W / 2], zmax = 0;
+        float top[2];
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int c = 0; c < 2; c++) {
+            top[c] = fmaxf(fmaxf(x[0][c], x[0][2 + c]), fmaxf(x[1][c], x[1][2 + c]));
 #pragma unroll
-            for (int r = 0; r < 2; r++)
-#pragma unroll
-                for (int i = 0; i < W / 2; i++) zmax = max_u16x2(zmax, vm[h][r].v[W / 2 + i] & 0x7fff7fffu);
-        zmax = __reduce_max_sync(0xffffffffu, max(zmax << 16, zmax));
-        const int more = max(static_cast<int>(zmax >> 23) - (127 + 95) - lift, 0);  // |z| from 2^95 on
-        lift += more;
+            for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+            top[c] = fmaxf(M[c], top[c]);
+            if (top[c] == -INFINITY) top[c] = 0.f;
+        }
+        uint32_t now[W / 2];
 #pragma unroll
         for (int i = 0; i < W / 2; i++) {
             const uint32_t m = max_u16x2(max_u16x2(vm[0][0].v[i], vm[0][1].v[i]), max_u16x2(vm[1][0].v[i], vm[1][1].v[i]));
             const uint32_t lo = __reduce_max_sync(0xffffffffu, m << 16), hi = __reduce_max_sync(0xffffffffu, m);
-            // exponent fields: 2^(9 + lift - e) for a scale in [2^e, 2^(e + 1)), e + 127 being the scale's own (0: GAIN_MAX)
-            const uint32_t want = 0x83808380u + lift * 0x800080u - (__byte_perm(lo, hi, 0x7632) & 0x7f807f80u);
-            now[i] = min_u16x2(min_u16x2(gain[i] + more * 0x800080u, GAIN_MAX), want);
-        }
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                uint32_t sg = 0x3f803f80u + lift * 0x800080u;  // a pair of 2^lift
-#pragma unroll
-                for (int i = 0; i < W / 2; i++)  // (a NaN is passed over)
-                    sg = kv4::as_u32(__hmax2(kv4::as_bf2(sg), kv4::as_bf2(mul_bf16x2(vm[h][r].v[i], now[i]))));
-                const float ls = __log2f(fmaxf(__uint_as_float(sg << 16), __uint_as_float(sg & 0xffff0000u)));
-                top[0] = fmaxf(top[0], fmaf(x[h][2 * r], Q.mul0, ls));
-                top[1] = fmaxf(top[1], fmaf(x[h][2 * r + 1], Q.mul1, ls));
-            }
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-            top[c] = fmaxf(M[c] + more, top[c] - 10.f);
-            if (top[c] == -INFINITY) top[c] = 0.f;
+            // exponent fields: 2^(21 - e) for a scale in [2^e, 2^(e + 1)), e + 127 being the scale's own (0: GAIN_MAX)
+            now[i] = min_u16x2(gain[i], 0x89808980u - (__byte_perm(lo, hi, 0x7632) & 0x7f807f80u));
         }
         if (M[0] != -INFINITY) {  // some sums there are
             float g[W];  // now / gain, 0 below 2^-149
@@ -417,7 +398,7 @@ struct State {
             for (int w = 0; w < W; w++) g[w] = pick(now, w) * __uint_as_float(0x7f000000u - __float_as_uint(pick(gain, w)));
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                const float f = fast_exp2(M[c] - top[c]);
+                const float f = fast_exp2((M[c] - top[c]) * (c ? Q.mul1 : Q.mul0));
 #pragma unroll
                 for (int i = 0; i < 2 * W; i++) {
                     acc[i][c] *= f * g[i / 2];
@@ -487,14 +468,14 @@ struct State {
             }
         }
     }
-    // The state as a record: m[8], l[8], o[8][HD].
-    __device__ __forceinline__ void record(float *R, int lane) {
+    // The state as a record: m[8] (base-2 logits), l[8], o[8][HD].
+    __device__ __forceinline__ void record(float *R, const Query<HD> &Q, int lane) {
         const int g = lane >> 2, t = lane & 3;
         float l[2], z[W][2];
         reduce(l, z, lane);
         if (g == 0) {
-            R[2 * t] = M[0];
-            R[2 * t + 1] = M[1];
+            R[2 * t] = M[0] * Q.mul0;
+            R[2 * t + 1] = M[1] * Q.mul1;
             R[GMAX + 2 * t] = l[0];
             R[GMAX + 2 * t + 1] = l[1];
         }
@@ -855,7 +836,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
             } else {
                 S.record(k == n ? reinterpret_cast<float *>(sm + warp * Y::RING)
                                 : reinterpret_cast<float *>(sm + Y::FIRST) + warp * Y::REC,
-                         lane);
+                         Q, lane);
             }
             if (k == n && warp == nb - 1 && lane == 0) cuts[nb] = Cut{ends ? -1 : s * nk + kh, Sg, Sg + T};
             j = 0;
@@ -970,11 +951,12 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         float m = cf + d4 <= cl ? __ldcg(at(cf + d4)) : -INFINITY;
         float lw = cf + d4 <= cl ? __ldcg(at(cf + d4) + GMAX) : 0.f;
         float M = m, l = 0.f;
+        constexpr float DOWN = 8.f;  // 2^-8 of everything: sums over a take's positions stay inside fp32
         for (int cc = cf + d4 + LPH; cc <= cl; cc += LPH) M = fmaxf(M, __ldcg(at(cc)));
 #pragma unroll
         for (int e = 1; e < LPH; e <<= 1) M = fmaxf(M, __shfl_xor_sync(mates, M, e, LPH));  // a head's threads come together
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        float f = fast_exp2(m - M);
+        float f = fast_exp2(m - M - DOWN);
         l = f * lw;
 #pragma unroll 1
         for (int c0 = cf;;) {
@@ -989,7 +971,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
             for (int e = 0; e < N; e++) v[e] = c0 + e <= cl ? numer(c0 + e) : make_float4(0.f, 0.f, 0.f, 0.f);
             if ((c0 - cf) % LPH == 0) {  // the next LPH records' references
                 const bool in = c0 + d4 <= cl;
-                f = in ? fast_exp2(__ldcg(at(c0 + d4)) - M) : 0.f;
+                f = in ? fast_exp2(__ldcg(at(c0 + d4)) - M - DOWN) : 0.f;
                 l = in ? fmaf(f, __ldcg(at(c0 + d4) + GMAX), l) : l;
             }
         }

@@ -982,7 +982,8 @@ int decode_kv4_entry(bool fused, const void *qkv, void *pool, void *out, void *h
                      const int *lens, int B, int nq, int nk, int hd, int npages, int maxpages, float scale,
                      oumu_stream_t stream) {
     if (!qkv || !pool || !out || !ws || !table || (!pos && !lens)) return OUMU_ERR_INVALID;
-    if (nq < 1 || nk < 1 || nq % nk || !(scale > 0.f)) return OUMU_ERR_INVALID;
+    const float sl2 = scale * 1.4426950408889634f;
+    if (nq < 1 || nk < 1 || nq % nk || !(scale > 0.f) || !std::isfinite(sl2)) return OUMU_ERR_INVALID;
     if ((cos_t == nullptr) != (sin_t == nullptr) || (cos_t && rot_rows < 1)) return OUMU_ERR_INVALID;
     int rc = paged_limits(B, npages, maxpages);
     if (rc) return rc;
@@ -1014,7 +1015,7 @@ int decode_kv4_entry(bool fused, const void *qkv, void *pool, void *out, void *h
     P.nk = nk;
     P.npages = npages;
     P.maxpages = maxpages;
-    P.sl2 = scale * 1.4426950408889634f;
+    P.sl2 = sl2;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return hd == 128 ? launch_decode_kv4<128>(fused, P, ws_bytes, sms, st)
                      : launch_decode_kv4<64>(fused, P, ws_bytes, sms, st);

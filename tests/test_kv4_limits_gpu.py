@@ -1,8 +1,9 @@
-"""The 4-bit paged cache at its limits: lengths that its tables do not hold, V of any size a bf16
-has, pools that run out."""
+"""The 4-bit paged cache at its limits: lengths that its tables do not hold, V and q of any size a
+bf16 has, pools that run out."""
 import pytest
 import torch
 
+import kv4_ref as ref
 from oumu_b200 import ops
 from oumu_b200.kv4 import KV4Cache
 from test_kv4_gpu import LENGTH, attn_case, check_attn, i32, randn, run_attn
@@ -104,6 +105,39 @@ def test_nan_in_a_group_of_v_stays_in_it(cuda, hd, group):
     big = float(kv[:, 1].abs().max())
     tol = 2 * (good.abs() * 2 ** -8 + 2 * big * (1 + 2 ** -7) * (2 ** -11 + 2 ** -14) + big * 2 ** -14)
     assert bool(((out - good).abs() <= tol)[~hit].all())
+
+
+# ---- q of any size ----
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("q_size,k_size", [(1e30, 1e-30), (1e32, 1e-32), (1e34, 1e-34), (1e33, 1.0),
+                                           (1e36, 1e-2), (1e5, 1.0), (1e8, 1.0), (1.0, 1e30), (1e-30, 1e30),
+                                           (1e-36, 1e36), (1e-38, 1.0)])
+def test_attention_with_q_of_any_size(cuda, q_size, k_size, hd):
+    nq, nk, lens = 8, 2, [300, 33]
+    kv = randn(98, 600, 2 * nk * hd).float().view(600, 2, nk, hd)
+    kv[:, 0] *= k_size
+    q = (randn(99, 2, nq * hd).float() * q_size).bfloat16()
+    qkv, pool, rows, table, ln = attn_case(lens, nq, nk, hd, seed=98, kv=kv.bfloat16().view(600, -1), q=q)
+    check_attn(run_attn(qkv, pool, table, ln, 2, nq, nk, hd), qkv, pool, rows, lens, nq, nk, hd)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_at_a_tiny_scale(cuda, hd):
+    """A scale that leaves nothing of the logits: the average of V, for q of 0 too."""
+    nq, nk, n = 4, 2, 45
+    qkv, pool, rows, table, ln = attn_case([n], nq, nk, hd, seed=100)
+    qkv[:, :hd] = 0
+    out = torch.empty(1, nq * hd, dtype=torch.bfloat16, device="cuda")
+    for scale in (1e-18, 1e-30, 1e-38):
+        ops.attn_decode_kv4(qkv, pool, out, ops.decode_kv4_workspace(1, nq, nk, hd, 1), table, None, ln, 1, nq, nk, hd,
+                            scale)
+        k, v, vs = ref.take_values(pool.cpu(), rows[0], n, nk, hd)
+        want = v.mean(1).repeat_interleave(2, 0)
+        # the bound of check_attn
+        tol = 15 * vs.amax(1) * (2 ** -11 + 2 ** -14) + v.abs().amax(1) * 2 ** -14
+        tol = want.abs() * 2 ** -8 + tol.repeat_interleave(2, 0)
+        assert bool(((out.cpu().double().view(nq, hd) - want).abs() <= tol).all())
 
 
 # ---- the cache's own calls ----
