@@ -94,7 +94,7 @@ __device__ __forceinline__ Quant quant_of(uint32_t range) {
     const float D = __fadd_ru(r.x, r.y);
     const uint32_t b = __float_as_uint(D * __uint_as_float(0x3d88888au)) & 0xffff0000u;
     q.s = __uint_as_float(15.f * __uint_as_float(b) >= D ? b : b + 0x10000u);
-    if (!(D < 3.4e38f)) q.s = __uint_as_float(0x7fc00000u);
+    if (!(D < INFINITY)) q.s = __uint_as_float(0x7fc00000u);
     q.rinv = __fdividef(1.f, q.s);
     // quant_pairs takes x - z as fp32 has it, which is exact for ordinary groups: where z is 0 or at least 2^-12 s, and x
     // too, both are multiples of 2^-19 of the power of two at or below s, and the difference is below 2^5 of it. Where x

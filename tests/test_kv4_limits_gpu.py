@@ -1,5 +1,5 @@
 """The 4-bit paged cache at its limits: lengths that its tables do not hold, V and q of any size a
-bf16 has, pools that run out."""
+bf16 has, spreads next to fp32's largest, pools that run out."""
 import pytest
 import torch
 
@@ -138,6 +138,23 @@ def test_attention_at_a_tiny_scale(cuda, hd):
         tol = 15 * vs.amax(1) * (2 ** -11 + 2 ** -14) + v.abs().amax(1) * 2 ** -14
         tol = want.abs() * 2 ** -8 + tol.repeat_interleave(2, 0)
         assert bool(((out.cpu().double().view(nq, hd) - want).abs() <= tol).all())
+
+
+# ---- spreads next to fp32's largest ----
+
+def test_groups_whose_spread_fp32_just_holds(cuda):
+    """max - min = 2^128 - 2^112: fp32 has it, so the group is held like any other."""
+    nk, hd = 1, 64
+    top, low = 2.0 ** 128 - 2.0 ** 120, -(2.0 ** 120 - 2.0 ** 112)
+    x = torch.linspace(0, 1, 32, dtype=torch.float64) * 2.0 ** 127
+    x[3], x[17] = top, low
+    x = x.float().bfloat16().repeat(4)
+    pool = torch.full((1, ref.page_bytes(nk, hd)), 255, dtype=torch.uint8, device="cuda")
+    ops.kv4_write(x.cuda(), pool, i32([[0]]), None, None, 1, 1, 0, nk, hd)
+    k, _, v, _ = ref.pool_values(pool.cpu(), nk, hd)
+    want = ref.held(x.view(2, 64).double())[3]
+    assert bool(torch.isfinite(want).all())
+    assert torch.equal(k[0, 0, 0], want[0]) and torch.equal(v[0, 0, 0], want[1])
 
 
 # ---- the cache's own calls ----
