@@ -10,8 +10,10 @@ from . import ops
 
 class KV4Cache:
     """`layers` layers of `npages` pages for B takes of up to maxlen positions. `lens` (int32 [B], device) holds the takes'
-    lengths; a caller that advances its own on the device (oumu_step_end) passes it. Everything is enqueued on the
-    current stream, without waiting for the GPU; calls to be captured take their takes as device tensors, not lists."""
+    lengths; a caller that advances its own on the device (oumu_step_end_live) passes it. Everything but `missing` is
+    enqueued on the current stream, without waiting for the GPU; calls to be captured take their takes as device tensors,
+    not lists. With programmatic launches on (ops.set_pdl), `step` and `attend` may start while the kernel before them
+    still runs: an ordinary launch (any of torch's) lies between free or compact and them (extend and fork end with one)."""
 
     def __init__(self, layers, B, nq, nk, hd, npages, maxlen, device="cuda", lens=None):
         self.layers, self.B, self.nq, self.nk, self.hd, self.npages = layers, B, nq, nk, hd, npages
@@ -32,7 +34,9 @@ class KV4Cache:
         self._pages_ws = ops.pages_workspace(npages, dev)
 
     def _ids(self, takes):
-        return torch.as_tensor(takes, dtype=torch.int32).to(self.table.device)
+        t = torch.as_tensor(takes, dtype=torch.int32)
+        # from pinned memory: a copy from pageable memory waits for the stream
+        return t if t.is_cuda else t.pin_memory().to(self.table.device, non_blocking=True)
 
     def extend(self, extra=0):
         """Pages for every take's first lens + extra positions. Those that the pool did not have are missing until

@@ -184,3 +184,19 @@ def test_pages_an_extend_lacked_stay_visible(cuda):
     c.free([0])
     c.extend()  # now there is a page, but the positions in between were not written
     assert c.missing() == 1 and c.missing() == 0
+
+
+def test_lists_of_takes_do_not_wait_for_the_gpu(cuda):
+    c = KV4Cache(1, 4, 8, 2, 64, 16, 256)
+    c.lens[0] = 70
+    c.extend()
+    c.fork([0], [1])
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    torch.cuda._sleep(400_000_000)  # some 0.2 s
+    c.fork([0], [2])
+    c.free([1])
+    done.record()
+    assert not done.query()
+    torch.cuda.synchronize()
+    assert c.lens.tolist() == [70, 0, 70, 0] and ops.device_error() == 0
