@@ -401,6 +401,8 @@ def _pools(pools, shape, ref):
 def pages_extend(table, ref, lens, extra, status):
     """Every take that holds positions gets the pages it lacks for lens[s] + extra of them (oumu_pages_extend);
     status[0]: pages missing."""
+    if not 0 <= extra < 1 << 31:  # ctypes would cut it to 32 bits
+        raise ValueError("extra: positions, below 2^31")
     dev, rows = torch.cuda.current_device(), table.shape
     _ints(dev, table, ref, lens, status)
     if len(rows) != 2 or lens.numel() < rows[0] or status.numel() < 1:
