@@ -65,6 +65,19 @@ class KV4Cache:
         """Pages in use to the front of the pools; moved = [pages in use, pages moved]."""
         ops.pages_compact(self.pools, self.table, self.ref, self._pages_ws, self.moved)
 
+    def resize(self, npages):
+        """`npages` pages from now on: those in use move to the front, into new pools, and the old pools' memory is free
+        again. Waits for the GPU; graphs captured before hold the old pools and have to be captured anew."""
+        self.compact()
+        used = int(self.moved[0])
+        if npages < max(used, 1):
+            raise ValueError(f"{used} pages are in use")
+        ws = ops.pages_workspace(npages, self.table.device)
+        pools, ref = self.pools.new_empty((self.layers, npages, self.pools.shape[2])), self.ref.new_zeros(npages)
+        pools[:, :used] = self.pools[:, :used]
+        ref[:used] = self.ref[:used]
+        self.pools, self.ref, self._pages_ws, self.npages = pools, ref, ws, npages
+
     def write(self, layer, qkv, rows, nq=None, start=None, count=None):
         """k and v of `rows` rows per take of qkv (nq q heads before them, by default the cache's) at start[s] + i."""
         ops.kv4_write(qkv, self.pools[layer], self.table, start, count, self.B, rows, self.nq if nq is None else nq,

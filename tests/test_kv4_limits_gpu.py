@@ -200,3 +200,38 @@ def test_lists_of_takes_do_not_wait_for_the_gpu(cuda):
     assert not done.query()
     torch.cuda.synchronize()
     assert c.lens.tolist() == [70, 0, 70, 0] and ops.device_error() == 0
+
+
+def test_a_cache_gives_its_free_pages_back_and_grows(cuda):
+    """Three of five takes are freed and the cache cut to what is left: its bytes shrink, the other takes' outputs stay; it
+    grows again when a take needs more."""
+    nq, nk, hd, layers, B = 8, 2, 64, 3, 5
+    c = KV4Cache(layers, B, nq, nk, hd, 24, 512)
+    c.lens.copy_(i32([300, 64, 130, 250, 190]))
+    c.extend()
+    for l in range(layers):
+        c.write(l, randn(110 + l, B * 300, 2 * nk * hd), 300, nq=0, count=c.lens)
+    qkv = randn(120, B, (nq + 2 * nk) * hd)
+
+    def outputs():
+        out = torch.empty(layers, B, nq * hd, dtype=torch.bfloat16, device="cuda")
+        for l in range(layers):
+            c.attend(l, qkv, out[l])
+        return out[:, [2, 4]]
+
+    c.free([0, 1, 3])
+    want, before = outputs(), c.nbytes()  # (the split of the work, and with it last bits, go by every take's length)
+    with pytest.raises(ValueError):
+        c.resize(5)  # 3 pages of each take are in use
+    assert torch.equal(outputs(), want)
+    c.resize(6)
+    assert c.npages == 6 and c.nbytes() * 4 == before and int((c.ref > 0).sum()) == 6
+    assert torch.equal(outputs(), want)
+    c.lens[2] = 193
+    c.extend()
+    assert c.missing() == 1
+    c.resize(9)
+    c.extend()
+    assert c.missing() == 0 and c.table[2].max().item() == 6
+    c.lens[2] = 130
+    assert torch.equal(outputs(), want) and ops.device_error() == 0
