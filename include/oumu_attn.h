@@ -252,9 +252,9 @@ int oumu_kv4_read(const void *pool, const int *table, const int *lens, const int
  * be of any size, and groups of 32 channels may differ in it as they like; a position whose V scale is
  * below 2^-23 of its group's largest in the take loses bits of its codes, which are as far below the group's others.
  * |q| scale stays below 2^117; an element of q below 2^-27 of its head's largest loses bits.
- * hd in {64, 128}, nq / nk in 1..8. The workspace is zero-filled before its first use, and before a use with another B or
- * nk (or oumu_attn_decode_reset with the new ones); every call leaves its counters zero, and calls that may overlap have
- * one each.
+ * hd in {64, 128}, nq / nk in 1..8. The workspace is zero-filled before its first use (or oumu_attn_decode_reset with the
+ * largest B and nk it will serve: one of a size serves every smaller shape), every call leaves its counters zero, and calls
+ * that may overlap have one each.
  */
 size_t oumu_attn_decode_kv4_workspace(int B, int nq, int nk, int hd, int maxpages);
 int oumu_attn_decode_kv4(const void *qkv, const void *pool, void *out, void *workspace, size_t workspace_bytes,

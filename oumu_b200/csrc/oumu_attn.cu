@@ -960,10 +960,13 @@ Kv4Cut kv4_cut(int B, long blocks, int nk, int sms, int large) {
 size_t kv4_part_bytes(int hd) { return 2 * (2 * static_cast<size_t>(d4::GMAX) + d4::GMAX * hd) * 4; }
 
 template <int HD, int NW>
-int launch_decode_kv4(bool fused, const d4::Params &P, size_t ws_bytes, int sms, cudaStream_t st) {
+int launch_decode_kv4(bool fused, d4::Params P, size_t ws_bytes, int sms, cudaStream_t st) {
     // one CTA per SM, fewer where the workspace holds fewer CTAs' records
     const long fit = static_cast<long>((ws_bytes - decode_counter_bytes(P.B, P.nk)) / kv4_part_bytes(HD));
     const unsigned grid = static_cast<unsigned>(std::min(static_cast<long>(sms), fit));
+    // the records at the workspace's end, so that where a larger batch has its counters stays zero
+    P.part = reinterpret_cast<float *>(reinterpret_cast<char *>(P.cnt) +
+                                       ((ws_bytes - grid * kv4_part_bytes(HD)) & ~static_cast<size_t>(15)));
     OUMU_CK(launch_k(fused ? d4::k_attn_decode_kv4<HD, NW, true> : d4::k_attn_decode_kv4<HD, NW, false>, dim3(grid),
                      dim3(NW * 32), d4::Lay<HD, NW>::bytes(P.B), st, P));
     return OUMU_OK;
@@ -1004,7 +1007,7 @@ int decode_kv4_entry(bool fused, const void *qkv, void *pool, void *out, void *h
     P.out = static_cast<bf16 *>(out);
     P.held = static_cast<bf16 *>(held);
     P.cnt = static_cast<int *>(ws);
-    P.part = reinterpret_cast<float *>(static_cast<char *>(ws) + cbytes);
+    P.part = nullptr;  // by the grid
     P.pos = pos;
     P.lens = lens;
     P.cos_t = cos_t;

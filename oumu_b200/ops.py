@@ -351,7 +351,7 @@ def kv4_read(pool, table, lens, kc, vc, nk, hd, pos=None):
 
 
 def decode_kv4_workspace(B, nq, nk, hd, maxpages, device=None):
-    """A zero-filled workspace for attn_decode_kv4 and attn_decode_kv4_step of this B and nk."""
+    """A zero-filled workspace for attn_decode_kv4 and attn_decode_kv4_step of this shape and smaller ones."""
     n = int(_lib.load().oumu_attn_decode_kv4_workspace(B, nq, nk, hd, maxpages))
     if n == 0:
         raise ValueError("unsupported decode shape")

@@ -157,6 +157,23 @@ def test_groups_whose_spread_fp32_just_holds(cuda):
     assert torch.equal(k[0, 0, 0], want[0]) and torch.equal(v[0, 0, 0], want[1])
 
 
+# ---- workspaces ----
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_one_workspace_for_batches_of_several_sizes(cuda, hd):
+    """Records of a smaller batch do not lie where a larger one has its counters."""
+    nq, nk = 8, 2
+    most = 1200
+    sizes = {2: [4000, 4007], most: [1 + s % 90 for s in range(most)], 40: [200 + 7 * s for s in range(40)]}
+    ws = ops.decode_kv4_workspace(most, nq, nk, hd, 64)
+    for B, lens in list(sizes.items()) * 2:
+        qkv, pool, rows, table, ln = attn_case(lens, nq, nk, hd, seed=B)
+        out = torch.full((B, nq * hd), float("nan"), dtype=torch.bfloat16, device="cuda")
+        ops.attn_decode_kv4(qkv, pool, out, ws, table, None, ln, B, nq, nk, hd, hd ** -0.5)
+        assert torch.equal(out, run_attn(qkv, pool, table, ln, B, nq, nk, hd))
+        assert int(ws[:4 * most * nk].int().sum()) == 0
+
+
 # ---- the cache's own calls ----
 
 def test_pages_a_fork_lacked_stay_visible(cuda):
