@@ -2,9 +2,10 @@
 // position's rope, quantisation and cache write in the same launch.
 //
 // Measured (one B200, back to back in a graph, 16 q and 2 kv heads of 128): 256 takes of 330..4096 positions, 184 MB,
-// 49.4 us (3.7 TB/s; the copies alone take 32); 64 takes 21.0 us; 32 takes 17.5; 2 takes of 65536 positions 21.0; one of
-// 512 8.3. Long caches stream at 6.3 TB/s, the rest is fixed: 3 us to the first tile, 3 to 4 from a CTA's last tile to
-// the end (merge, counter, the last one's sum), 2 of launch, and what the warps' ends differ by.
+// 49 us (3.8 TB/s; the copies alone take 32); 64 takes 21.2 us; 32 takes 17.6; 2 takes of 65536 positions 21.7; one of
+// 512 8.4. 64 takes of 24576 positions, 504 MB, take 92.4 us (5.5 TB/s), of 8192 41.1 (4.1): 6.5 TB/s between the two,
+// the rest is fixed: 3 us to the first tile, 3 to 4 from a CTA's last tile to the end (merge, counter, the last one's
+// sum), 2 of launch, and what the warps' ends differ by.
 //
 // The mathematics. With value = s n + z for each group of 32 channels,
 //   score_j = sum_g s_jg (q . n_j)_g + sum_g z_jg Q_g,    Q_g = the sum of q over group g,
@@ -577,8 +578,8 @@ struct Newest {
 // adds them up in CTA order: the result does not depend on timing.
 //
 // NW warps and ST tiles in flight for each. 12 warps keep three per scheduler, which hides more of the instructions'
-// latencies (5 KB of cache take about 650 instructions): 6.3 TB/s on long caches against 5.2 with 8, of 7.1 for the copies
-// alone. 8 warps have less to merge at the end (the launch's rule has both sides' times).
+// latencies (5 KB of cache take about 660 instructions): between 64 takes of 8192 and of 24576 positions they stream at
+// 6.3 TB/s against 5.2 with 8, of 7.1 for the copies alone. 8 warps have less to merge at the end (the launch's rule has both sides' times).
 template <int HD>
 constexpr int TP = HD == 128 ? kv4::HALF : kv4::PAGE;  // positions per tile
 template <int NW>
@@ -732,7 +733,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attn_decode_kv4(Params P) {
         return;
     }
     const Parts parts(tb - ta, NW);
-    // by way of a shuffle: the loop then takes 3 to 12 registers fewer (long caches 6.26 TB/s, 6.05 without)
+    // by way of a shuffle: the loop then takes 3 to 12 registers fewer (6.26 TB/s between 64 takes of
+    // 8192 and of 24576 positions, 6.05 without)
     const int bound = ta + parts.start(warp + (lane & 1));
     const int wa = __shfl_sync(0xffffffffu, bound, 0), wb = __shfl_sync(0xffffffffu, bound, 1), n = wb - wa;
 

@@ -376,8 +376,8 @@ struct WriteTo {
 
 // 512 bytes are read and 160 written per position and kv head at hd 128; the quantiser's instructions (69 % of the issue
 // slots) bound it as much as HBM. The lanes load row chunks in the order of the block's words, so a block's 512 bytes of
-// codes leave in one 16-byte store per lane. 48 prompts of 427..4048 positions, 145 MB: 42 us (3.5 TB/s); one prompt of
-// 1024: 3.7 us.
+// codes leave in one 16-byte store per lane. 48 prompts of 427..4048 positions, 145 MB: 42.5 us (3.4 TB/s); one prompt of
+// 1024: 4.0 us. At hd 128 the 80 registers that three CTAs an SM leave spill 24 bytes a thread.
 template <int HD>
 __global__ void __launch_bounds__(256, 3) k_kv4_write(const bf16 *qkv, uint8_t *pool, const int *table, const int *start,
                                                    const int *count, int B, int rows, int nq, int nk, int npages,
@@ -436,7 +436,7 @@ __device__ __forceinline__ float value_of(uint32_t half, int i, float s, float z
 }
 
 // The write's order backwards; a part's codes and meta rows are all loaded before the first value is stored. Bound by HBM:
-// the 48 prompts above in 27.4 us (5.4 TB/s).
+// the 48 prompts above, with 77 positions before each 150 MB, in 27.4 us (5.5 TB/s).
 template <int HD, int PER>
 __global__ void __launch_bounds__(256) k_kv4_read(uint8_t *pool, const int *table, const int *lens, const int *pos,
                                                   bf16 *kc, bf16 *vc, int B, int nk, int npages, int maxpages,

@@ -972,7 +972,8 @@ int launch_decode_kv4(bool fused, d4::Params P, size_t ws_bytes, int sms, cudaSt
     return OUMU_OK;
 }
 // 12 warps where full tables would give 8 warps an SM 10 tiles each, or more (lengths are known on the device only). 8 | 12
-// warps: 256 takes of up to 4096 positions 53.3 | 49.2 us, 64 takes 21.9 | 21.3, 32 takes 17.3 | 18.3, one of 512 8.4 | 9.5.
+// warps: 256 takes of up to 4096 positions 53.3 | 49.2 us, 64 takes 21.9 | 21.3, 32 takes 17.3 | 18.3, one of 512 8.4 | 9.5
+// (so a table far wider than its takes are long costs them up to 1 us).
 template <int HD>
 int launch_decode_kv4(bool fused, const d4::Params &P, size_t ws_bytes, int sms, cudaStream_t st) {
     const long tiles = static_cast<long>(P.B) * P.nk * P.maxpages * (kv4::PAGE / d4::TP<HD>);

@@ -4,8 +4,8 @@
 // Whoever hands out or moves pages works in one block, in the order of takes and page numbers (prefix sums, no race
 // decides), so the same state gives the same pages in every run; what copies bytes runs on the whole GPU. The counts
 // and tables are a few KB, so these launches are bound by their latency, the copies by HBM. Measured on one B200: 64 takes
-// forked from a prompt of 1000 positions in 36 layers and extended 17.9 us (47 MB written), 248 of 1000 pages of 36 layers
-// moved in 68.6 us (366 MB, 5.3 TB/s).
+// forked from a prompt of 1000 positions in 36 layers and extended 18.0 us (47 MB written; the extend 2.1), freed 1.7 us,
+// 248 of 1000 pages of 36 layers moved in 67.6 us (366 MB, 5.4 TB/s).
 #pragma once
 #include "common.cuh"
 #include "kv4.cuh"
