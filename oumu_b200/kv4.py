@@ -76,6 +76,7 @@ class KV4Cache:
         pools, ref = self.pools.new_empty((self.layers, npages, self.pools.shape[2])), self.ref.new_zeros(npages)
         pools[:, :used] = self.pools[:, :used]
         ref[:used] = self.ref[:used]
+        torch.cuda.synchronize(self.table.device)  # other streams may still read the old pools
         self.pools, self.ref, self._pages_ws, self.npages = pools, ref, ws, npages
 
     def write(self, layer, qkv, rows, nq=None, start=None, count=None):

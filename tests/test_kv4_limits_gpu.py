@@ -252,3 +252,34 @@ def test_a_cache_gives_its_free_pages_back_and_grows(cuda):
     assert c.missing() == 0 and c.table[2].max().item() == 6
     c.lens[2] = 130
     assert torch.equal(outputs(), want) and ops.device_error() == 0
+
+
+def test_extend_and_fork_then_step_with_programmatic_launches(cuda):
+    """No launch of the caller's between page calls and steps: the cache's own is one."""
+    nq, nk, hd, layers, B = 16, 2, 128, 2, 6
+    cs, sn = (t.cuda() for t in ops.rotary_tables(512, hd))
+    qkv = randn(130, 12, B, (nq + 2 * nk) * hd)
+    src, dst = i32([0, 0]), i32([4, 5])
+    results = []
+    for pdl in (False, True):
+        c = KV4Cache(layers, B, nq, nk, hd, 60, 512)
+        c.lens.copy_(i32([127, 64, 1, 300, 0, 0]))
+        c.extend()
+        for l in range(layers):
+            c.write(l, randn(131 + l, B * 300, 2 * nk * hd), 300, nq=0, count=c.lens)
+        out = torch.zeros(12, layers, B, nq * hd, dtype=torch.bfloat16, device="cuda")
+        torch.cuda.synchronize()
+        prev = ops.set_pdl(pdl)
+        try:
+            for i in range(12):
+                if i == 5:
+                    c.fork(src, dst)
+                c.lens.add_((c.lens > 0).int())
+                c.extend()
+                for l in range(layers):
+                    c.step(l, qkv[i], out[i, l], cs, sn)
+        finally:
+            ops.set_pdl(prev)
+        assert c.missing() == 0 and ops.device_error() == 0
+        results.append((out, c.table.clone(), c.lens.tolist()))
+    assert all(torch.equal(a, b) for a, b in zip(results[0][:2], results[1][:2])) and results[0][2] == results[1][2]
